@@ -10,7 +10,8 @@ from . import _lib
 from . import event
 from . import nn
 from . import host
+from . import plastic
 from .event import EventArray, FixedPostNumConn, CSR, FixedPreNumConn, CSC
 
 __version__ = '0.1.0'
-__all__ = ['event', 'nn', 'host', 'EventArray', 'FixedPostNumConn', 'CSR', 'FixedPreNumConn', 'CSC']
+__all__ = ['event', 'nn', 'host', 'plastic', 'EventArray', 'FixedPostNumConn', 'CSR', 'FixedPreNumConn', 'CSC']

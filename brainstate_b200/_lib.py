@@ -24,6 +24,7 @@ BSX_ERR_NONFINITE = -7
 VECMAT_GLOBAL_ATOMICS, VECMAT_SHARED_SLICES = 0, 1
 LINK_EARLY_PUSH, LINK_FETCH_AHEAD, LINK_DEFAULT = 1, 2, 3
 SPK_BOOL8, SPK_F32, SPK_BITS32, SPK_LIST = 0, 1, 2, 3
+T_F32, T_BF16, T_F16 = 0, 1, 2
 
 
 class BsxError(RuntimeError):
@@ -84,10 +85,24 @@ class BsxNetLinks(C.Structure):
                 ('spin_limit', C.c_int64), ('seq0', C.c_int64), ('inbox', C.c_void_p * 16), ('sync', C.c_void_p), ('flags', C.c_int32)]
 
 
+class BsxDelta(C.Structure):
+    """Mirror of ``bsx_delta_t``."""
+    _fields_ = [
+        ('batch', C.c_int64), ('tokens', C.c_int64),
+        ('k_heads', C.c_int32), ('v_heads', C.c_int32), ('dk', C.c_int32), ('dv', C.c_int32),
+        ('dtype', C.c_int32), ('scale', C.c_float),
+        ('q', C.c_void_p), ('k', C.c_void_p), ('v', C.c_void_p), ('g', C.c_void_p), ('beta', C.c_void_p),
+        ('initial', C.c_void_p), ('lengths', C.c_void_p),
+        ('q_stride', C.c_int64 * 3), ('k_stride', C.c_int64 * 3), ('v_stride', C.c_int64 * 3),
+        ('g_stride', C.c_int64 * 3), ('beta_stride', C.c_int64 * 3),
+    ]
+
+
 _i64, _i32, _vp, _sz, _f32 = C.c_int64, C.c_int, C.c_void_p, C.c_size_t, C.c_float
 _connp = C.POINTER(BsxConn)
 _netp = C.POINTER(BsxNet)
 _lifp = C.POINTER(BsxLifParams)
+_deltap = C.POINTER(BsxDelta)
 
 # name -> (restype, argtypes); every symbol include/bsx.h declares, plus the two tuning hooks of
 # csrc/bsx_tuning.h (INTERNAL lists them)
@@ -150,6 +165,11 @@ SIGNATURES = {
     'bsx_ipc_close': (_i32, [_vp]),
     'bsx_ipc_free': (_i32, [_vp]),
     'bsx_drive_hash': (C.c_uint32, [C.c_uint32, C.c_uint32, C.c_uint32]),
+    'bsx_delta_workspace_bytes': (_sz, [_deltap]),
+    'bsx_delta_forward': (_i32, [_deltap, _vp, _vp, _vp, _sz, _vp]),
+    'bsx_delta_recurrent': (_i32, [_deltap, _vp, _vp, _vp]),
+    'bsx_delta_backward_workspace_bytes': (_sz, [_deltap]),
+    'bsx_delta_backward': (_i32, [_deltap, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     'bsx_fill_f32': (_i32, [_vp, _i64, _f32, _vp]),
 }
 

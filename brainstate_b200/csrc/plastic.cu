@@ -1,0 +1,152 @@
+// Gated delta rule: C entry points, argument checks and the layout of the workspace.
+#include "plastic.cuh"
+
+namespace bsx {
+namespace plastic {
+
+int launch_step(const Args& a, int dtype, cudaStream_t st);
+
+static int64_t chunks_of(int64_t tokens) { return (tokens + kC - 1) / kC; }
+static int width_of(int dk) { return dk <= 64 ? 64 : 128; }
+
+static size_t workspace(const bsx_delta_t* d, bool backward) {
+  const int64_t n = d->batch * d->v_heads * chunks_of(d->tokens);
+  size_t f = (size_t)n * (2 * kC * kC + kVec);
+  if (backward) {
+    f += (size_t)n * (kC * kC + 2 * (size_t)d->dv * (width_of(d->dk) + kC));
+    if (d->k_heads != d->v_heads) f += 2 * (size_t)d->batch * d->tokens * d->v_heads * d->dk;
+  }
+  return f * sizeof(float);
+}
+
+static int check_sizes(const bsx_delta_t* d) {
+  if (!d) return fail(BSX_ERR_INVALID_ARG, "description is NULL");
+  if (d->batch < 0 || d->tokens < 0) return fail(BSX_ERR_INVALID_ARG, "negative size");
+  if (d->dtype < BSX_T_F32 || d->dtype > BSX_T_F16) return fail(BSX_ERR_INVALID_ARG, "unknown element type");
+  if (d->k_heads < 1 || d->v_heads < 1 || d->v_heads % d->k_heads != 0)
+    return fail(BSX_ERR_INVALID_ARG, "v_heads must be a positive multiple of k_heads");
+  if (d->dk < 1 || d->dv < 1) return fail(BSX_ERR_INVALID_ARG, "dk and dv must be positive");
+  if (d->dk > 128) return fail(BSX_ERR_UNSUPPORTED, "dk above 128");
+  if (d->dv > 4096) return fail(BSX_ERR_UNSUPPORTED, "dv above 4096");
+  if (d->tokens > INT32_MAX - kC || d->batch > INT32_MAX) return fail(BSX_ERR_UNSUPPORTED, "batch and tokens must fit int32");
+  const int64_t blocks_per_head = chunks_of(d->tokens) > (d->dv + 15) / 16 ? chunks_of(d->tokens) : (d->dv + 15) / 16;
+  if (d->batch > 0 && d->v_heads > INT32_MAX / blocks_per_head / d->batch)
+    return fail(BSX_ERR_UNSUPPORTED, "batch * v_heads * chunks must fit int32");
+  return BSX_OK;
+}
+
+static int fill(const bsx_delta_t* d, Args& a) {
+  int rc = check_sizes(d);
+  if (rc != BSX_OK) return rc;
+  if (d->batch > 0 && d->tokens > 0 && (!d->q || !d->k || !d->v || !d->g || !d->beta))
+    return fail(BSX_ERR_INVALID_ARG, "NULL input");
+  a = Args{};
+  a.q = d->q; a.k = d->k; a.v = d->v; a.g = d->g; a.beta = d->beta;
+  a.initial = d->initial; a.lengths = d->lengths;
+  for (int i = 0; i < 3; ++i) {
+    a.qs[i] = d->q_stride[i]; a.ks[i] = d->k_stride[i]; a.vs[i] = d->v_stride[i];
+    a.gs[i] = d->g_stride[i]; a.bs[i] = d->beta_stride[i];
+  }
+  a.T = d->tokens; a.B = (int)d->batch; a.Hk = d->k_heads; a.Hv = d->v_heads; a.dk = d->dk; a.dv = d->dv;
+  a.NC = (int)chunks_of(d->tokens);
+  a.scale = d->scale;
+  const int per = d->dtype == BSX_T_F32 ? 4 : 8;     // elements of a 16-byte stretch
+  auto vec = [per](const void* p, const int64_t* s, int cols) {
+    return aligned16(p) && s[0] % per == 0 && s[1] % per == 0 && s[2] % per == 0 && cols % per == 0;
+  };
+  a.vec_qk = vec(a.q, a.qs, a.dk) && vec(a.k, a.ks, a.dk);
+  a.vec_v = vec(a.v, a.vs, a.dv);
+  return BSX_OK;
+}
+
+static void place(Args& a, const bsx_delta_t* d, float* ws, bool backward) {
+  const int64_t n = (int64_t)a.B * a.Hv * a.NC;
+  a.Tm = ws; ws += n * kC * kC;
+  a.Pm = ws; ws += n * kC * kC;
+  a.vec = ws; ws += n * kVec;
+  if (!backward) return;
+  const int64_t wide = width_of(a.dk);
+  a.Bm = ws; ws += n * kC * kC;
+  a.Sn = ws; ws += n * a.dv * wide;
+  a.dS = ws; ws += n * a.dv * wide;
+  a.U = ws; ws += n * a.dv * kC;
+  a.dY = ws; ws += n * a.dv * kC;
+  if (a.Hk != a.Hv) {
+    a.dq32 = ws; ws += (int64_t)a.B * a.T * a.Hv * a.dk;
+    a.dk32 = ws;
+  }
+}
+
+}  // namespace plastic
+}  // namespace bsx
+
+using namespace bsx;
+using namespace bsx::plastic;
+
+extern "C" size_t bsx_delta_workspace_bytes(const bsx_delta_t* d) {
+  return check_sizes(d) == BSX_OK ? workspace(d, false) : 0;
+}
+extern "C" size_t bsx_delta_backward_workspace_bytes(const bsx_delta_t* d) {
+  return check_sizes(d) == BSX_OK ? workspace(d, true) : 0;
+}
+
+extern "C" int bsx_delta_forward(const bsx_delta_t* d, void* out, float* state, void* ws, size_t ws_bytes,
+                                 bsx_stream_t stream) {
+  BSX_TRACE("bsx_delta_forward");
+  Args a;
+  int rc = fill(d, a);
+  if (rc != BSX_OK) return rc;
+  if (a.B == 0) return BSX_OK;
+  if (a.NC > 0 && !out) return fail(BSX_ERR_INVALID_ARG, "out is NULL");
+  if (a.NC == 0 && !state) return BSX_OK;
+  if (a.NC > 0 && (!ws || !aligned16(ws) || ws_bytes < workspace(d, false)))
+    return fail(BSX_ERR_WORKSPACE, "workspace missing, misaligned or too small");
+  if (sm_count() <= 0) return fail(BSX_ERR_CUDA, "no CUDA device");
+  a.o = out;
+  a.state = state;
+  place(a, d, static_cast<float*>(ws), false);
+  cudaStream_t st = as_stream(stream);
+  if (a.NC > 0 && (rc = launch_prepare(a, d->dtype, false, st)) != BSX_OK) return rc;
+  return launch_scan(a, d->dtype, false, st);
+}
+
+extern "C" int bsx_delta_recurrent(const bsx_delta_t* d, void* out, float* state, bsx_stream_t stream) {
+  BSX_TRACE("bsx_delta_recurrent");
+  Args a;
+  int rc = fill(d, a);
+  if (rc != BSX_OK) return rc;
+  if (a.B == 0) return BSX_OK;
+  if (a.T > 0 && !out) return fail(BSX_ERR_INVALID_ARG, "out is NULL");
+  if (a.T == 0 && !state) return BSX_OK;
+  if (sm_count() <= 0) return fail(BSX_ERR_CUDA, "no CUDA device");
+  a.o = out;
+  a.state = state;
+  return launch_step(a, d->dtype, as_stream(stream));
+}
+
+extern "C" int bsx_delta_backward(const bsx_delta_t* d, const void* dout, const float* dstate, void* dq, void* dk,
+                                  void* dv, float* dg, float* dbeta, float* dinitial, void* ws, size_t ws_bytes,
+                                  bsx_stream_t stream) {
+  BSX_TRACE("bsx_delta_backward");
+  Args a;
+  int rc = fill(d, a);
+  if (rc != BSX_OK) return rc;
+  if (a.B == 0) return BSX_OK;
+  if (a.NC > 0 && (!dout || !dq || !dk || !dv || !dg || !dbeta)) return fail(BSX_ERR_INVALID_ARG, "NULL buffer");
+  if (a.NC == 0 && !dinitial) return BSX_OK;
+  if (a.NC > 0 && (!ws || !aligned16(ws) || ws_bytes < workspace(d, true)))
+    return fail(BSX_ERR_WORKSPACE, "workspace missing, misaligned or too small");
+  if (sm_count() <= 0) return fail(BSX_ERR_CUDA, "no CUDA device");
+  a.dout = dout; a.dstate = dstate;
+  a.dq = dq; a.dk_ = dk; a.dv_ = dv; a.dg = dg; a.dbeta = dbeta; a.dinitial = dinitial;
+  const int per = d->dtype == BSX_T_F32 ? 4 : 8;
+  a.vec_do = aligned16(dout) && a.dv % per == 0;
+  place(a, d, static_cast<float*>(ws), true);
+  cudaStream_t st = as_stream(stream);
+  if (a.NC > 0) {
+    if ((rc = launch_prepare(a, d->dtype, true, st)) != BSX_OK) return rc;
+    if ((rc = launch_scan(a, d->dtype, true, st)) != BSX_OK) return rc;
+  }
+  if ((rc = launch_backward_scan(a, d->dtype, st)) != BSX_OK) return rc;
+  return a.NC > 0 ? launch_backward_chunks(a, d->dtype, st) : BSX_OK;
+}

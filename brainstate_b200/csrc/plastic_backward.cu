@@ -1,0 +1,783 @@
+// Gated delta rule, reverse mode.
+//
+// backward_scan_kernel: the pass over the chunks from the last to the first that carries the cotangent of the state,
+// in the same register form as the forward pass (16 value columns a group, transposed, accumulators used as left
+// operands).  With dS the cotangent of the state after the chunk:
+//   dU = P^T dO + diag(e^{G_C-G}) K dS,  dY = T^T dU,  dV = beta dY,  dR = -beta e^G dY,
+//   dS <- e^{G_C} dS + Q^T (scale e^G dO) + K^T dR.
+// It leaves dS (before the update) and dY for every chunk.
+//
+// backward_chunk_kernel: everything else, all chunks at once, one block per (row, head, chunk).  Over blocks of 32 value
+// columns it sums D1 = dY S0^T, Dq = dO S0^T, D3 = U dS^T (64 x dk) and dP = dO U^T, dA = -dY U^T (64 x 64), then
+//   dQ = scale e^G Dq + E K,                         E = scale Gamma dP (j <= i)
+//   dK = -beta e^G D1 + e^{G_C-G} D3 + E^T Q + (F + F^T) K,   F = beta Gamma dA (j < i)
+//   dbeta_i = dY_i.V_i - e^{G_i} K_i.D1_i + sum_j dA_ij (A/beta)_ij
+//   dG_i = -beta e^G K_i.D1_i + scale e^G Q_i.Dq_i - e^{G_C-G} K_i.D3_i + (row - column sums of dP P + dA A)_i,
+//   dG_C += sum_i e^{G_C-G_i} K_i.D3_i + e^{G_C} <S0, dS>,   dg = sums of dG from the chunk's end.
+#include "plastic.cuh"
+
+namespace bsx {
+namespace plastic {
+
+// ------------------------------------------------------------------------------------------------ pass over chunks
+
+template <typename E, int DK>
+struct BackScanLayout {
+  static constexpr int PK = DK + 8, PT = kC + 8, PP = kC + 4;   // T^T and P are read by column: PP
+  static constexpr size_t tile = (size_t)kC * PK * sizeof(E);
+  static constexpr size_t tri = (size_t)kC * PP * sizeof(float);
+  static constexpr int stages = (sizeof(E) == 4 && DK == 128) ? 1 : 2;
+  static constexpr size_t q_off = tile, t_off = 2 * tile, p_off = t_off + tri, vec_off = p_off + tri,
+                          v_off = vec_off + 3 * kC * sizeof(float);
+  static size_t v_bytes(int groups) { return (size_t)kC * (groups * 16 + 8) * sizeof(E); }
+  static size_t red_bytes(int groups, int ws) { return ws > 1 ? (size_t)groups * ws * 32 * 32 * 4 : 0; }
+  static size_t bytes(int groups, int ws) { return stages * (v_off + v_bytes(groups)) + red_bytes(groups, ws); }
+};
+
+template <typename E, int DK, int WS>
+__global__ void __launch_bounds__(256) backward_scan_kernel(Args a, int groups) {
+  using L = BackScanLayout<E, DK>;
+  constexpr bool X = IsExact<E>::value;
+  constexpr int DKW = DK / WS, NT = DKW / 8, NB = NT < 4 ? NT : 4;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int tid = threadIdx.x, nthr = blockDim.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int grp = warp / WS, w = warp - grp * WS;
+  const int per_head = (a.dv + 16 * groups - 1) / (16 * groups);
+  const int bh = blockIdx.x / per_head, vb = (blockIdx.x - bh * per_head) * groups * 16;
+  const int b = bh / a.Hv, h = bh - b * a.Hv, hk = h / (a.Hv / a.Hk);
+  const int len = row_length(a, b), nc = (len + kC - 1) / kC;
+  const int PV = groups * 16 + 8;
+  const size_t set = L::v_off + (size_t)kC * PV * sizeof(E);
+  float* red = reinterpret_cast<float*>(smem + L::stages * set);
+  const int d0 = vb + grp * 16 + g;
+  const int kb = w * DKW;
+
+  const E* kp = static_cast<const E*>(a.k) + b * a.ks[0] + hk * a.ks[2];
+  const E* qp = static_cast<const E*>(a.q) + b * a.qs[0] + hk * a.qs[2];
+  const int64_t os = (int64_t)a.Hv * a.dv;      // token stride of the outputs and their cotangents
+  const E* dop = static_cast<const E*>(a.dout) + (int64_t)b * a.T * os + (int64_t)h * a.dv + vb;
+
+  float s[NT][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int kr = kb + n * 8 + 2 * t + (i & 1), d = d0 + (i >> 1) * 8;
+      s[n][i] = (a.dstate && kr < a.dk && d < a.dv) ? a.dstate[((int64_t)bh * a.dk + kr) * a.dv + d] : 0.f;
+    }
+
+  auto load = [&](int c, int buf) {
+    unsigned char* base = smem + buf * set;
+    const int64_t t0 = (int64_t)c * kC;
+    const int rows = min(kC, len - c * kC);
+    const int64_t ci = (int64_t)bh * a.NC + c;
+    stage(reinterpret_cast<E*>(base), L::PK, kp + t0 * a.ks[1], a.ks[1], rows, a.dk, DK, a.vec_qk, tid, nthr);
+    stage(reinterpret_cast<E*>(base + L::q_off), L::PK, qp + t0 * a.qs[1], a.qs[1], rows, a.dk, DK, a.vec_qk, tid, nthr);
+    stage_lower(reinterpret_cast<float*>(base + L::t_off), L::PP, a.Tm + ci * kC * kC, tid, nthr);
+    stage_lower(reinterpret_cast<float*>(base + L::p_off), L::PP, a.Pm + ci * kC * kC, tid, nthr);
+    for (int i = tid; i < 3 * kC / 4; i += nthr)
+      cp16(base + L::vec_off + i * 16, a.vec + ci * kVec + i * 4, true);
+    stage(reinterpret_cast<E*>(base + L::v_off), PV, dop + t0 * os, os, rows, min(a.dv - vb, groups * 16), groups * 16,
+          a.vec_do, tid, nthr);
+    cp_commit();
+  };
+
+  if (L::stages == 2 && nc > 0) load(nc - 1, (nc - 1) & 1);
+  for (int c = nc - 1; c >= 0; --c) {
+    const int buf = L::stages == 2 ? (c & 1) : 0;
+    if (L::stages == 2) {
+      if (c > 0) {
+        load(c - 1, buf ^ 1);
+        cp_wait<1>();
+      } else {
+        cp_wait<0>();
+      }
+    } else {
+      load(c, 0);
+      cp_wait<0>();
+    }
+    __syncthreads();
+    const unsigned char* base = smem + buf * set;
+    const E* K = reinterpret_cast<const E*>(base);
+    const E* Q = reinterpret_cast<const E*>(base + L::q_off);
+    const float* Tm = reinterpret_cast<const float*>(base + L::t_off);
+    const float* Pm = reinterpret_cast<const float*>(base + L::p_off);
+    const float* eG = reinterpret_cast<const float*>(base + L::vec_off);
+    const float* eD = eG + kC;
+    const float* beta = eG + 2 * kC;
+    const E* DO = reinterpret_cast<const E*>(base + L::v_off) + grp * 16;
+    const int64_t ci = (int64_t)bh * a.NC + c;
+    const int64_t t0 = (int64_t)c * kC;
+
+    {
+      float* out = a.dS + ci * a.dv * DK;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+          if (d0 + 8 * hf < a.dv)
+            *reinterpret_cast<float2*>(out + (int64_t)(d0 + 8 * hf) * DK + kb + n * 8 + 2 * t) =
+                make_float2(s[n][2 * hf], s[n][2 * hf + 1]);
+    }
+
+    // dS^T K^T over this warp's key rows, scaled by e^{G_C-G}
+    float r[8][4];
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[n][i] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < NT; ++ks) {
+      float x[4], hi[4], lo[4];
+      as_left(s[ks], x);
+      split4(x, hi, lo);
+      float2 kk[8];
+#pragma unroll
+      for (int n = 0; n < 8; ++n) kk[n] = pair(K + (n * 8 + g) * L::PK + kb + ks * 8 + 2 * t);
+      mma_split<X, 8>(r, hi, lo, kk);
+    }
+    if (WS > 1) {
+      float* mine = red + (size_t)grp * WS * 32 * 32 + lane;   // free since the barrier at the chunk's end
+#pragma unroll
+      for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mine[(w * 32 + n * 4 + i) * 32] = r[n][i];
+      asm volatile("bar.sync %0, %1;" ::"r"(grp + 1), "n"(WS * 32) : "memory");
+#pragma unroll
+      for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float x = mine[(n * 4 + i) * 32];
+#pragma unroll
+          for (int p = 1; p < WS; ++p) x += mine[(p * 32 + n * 4 + i) * 32];
+          r[n][i] = x;
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      const float2 ed = pair(eD + n * 8 + 2 * t);
+      r[n][0] *= ed.x;
+      r[n][1] *= ed.y;
+      r[n][2] *= ed.x;
+      r[n][3] *= ed.y;
+    }
+    // dO^T (value columns as rows), then dU^T = dO^T P + ...
+    float x[8][4];
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[n][i] = to_f<E>(DO[(n * 8 + 2 * t + (i & 1)) * PV + g + 8 * (i >> 1)]);
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) {
+      float y[4], hi[4], lo[4];
+      as_left(x[ks], y);
+      if (!X) split4(y, hi, lo);
+      float2 ph[8], pl[8];
+#pragma unroll
+      for (int n = 0; n <= ks; ++n) {
+        const float* p = Pm + (ks * 8 + 2 * t) * L::PP + n * 8 + g;
+        split(p[0], ph[n].x, pl[n].x);
+        split(p[L::PP], ph[n].y, pl[n].y);
+      }
+      if (X) {
+#pragma unroll
+        for (int n = 0; n <= ks; ++n) mma(r[n], y, pl[n].x, pl[n].y);
+#pragma unroll
+        for (int n = 0; n <= ks; ++n) mma(r[n], y, ph[n].x, ph[n].y);
+      } else {
+#pragma unroll
+        for (int n = 0; n <= ks; ++n) mma(r[n], lo, ph[n].x, ph[n].y);
+#pragma unroll
+        for (int n = 0; n <= ks; ++n) mma(r[n], hi, pl[n].x, pl[n].y);
+#pragma unroll
+        for (int n = 0; n <= ks; ++n) mma(r[n], hi, ph[n].x, ph[n].y);
+      }
+    }
+    // dY^T = dU^T T
+    float dy[8][4];
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) dy[n][i] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) {
+      float y[4], hi[4], lo[4];
+      as_left(r[ks], y);
+      split4(y, hi, lo);
+      float2 th[8], tl[8];
+#pragma unroll
+      for (int n = 0; n <= ks; ++n) {
+        const float* p = Tm + (ks * 8 + 2 * t) * L::PP + n * 8 + g;
+        split(p[0], th[n].x, tl[n].x);
+        split(p[L::PP], th[n].y, tl[n].y);
+      }
+#pragma unroll
+      for (int n = 0; n <= ks; ++n) mma(dy[n], lo, th[n].x, th[n].y);
+#pragma unroll
+      for (int n = 0; n <= ks; ++n) mma(dy[n], hi, tl[n].x, tl[n].y);
+#pragma unroll
+      for (int n = 0; n <= ks; ++n) mma(dy[n], hi, th[n].x, th[n].y);
+    }
+    if (w == 0) {
+      float* Y = a.dY + ci * a.dv * kC;
+      E* dv = static_cast<E*>(a.dv_) + ((int64_t)b * a.T + t0) * os + (int64_t)h * a.dv;
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const int tok = n * 8 + 2 * t;
+        const float2 be = pair(beta + tok);
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const int d = d0 + 8 * hf;
+          if (d >= a.dv) continue;
+          *reinterpret_cast<float2*>(Y + (int64_t)d * kC + tok) = make_float2(dy[n][2 * hf], dy[n][2 * hf + 1]);
+          if (t0 + tok < len) dv[tok * os + d] = from_f<E>(be.x * dy[n][2 * hf]);
+          if (t0 + tok + 1 < len) dv[(tok + 1) * os + d] = from_f<E>(be.y * dy[n][2 * hf + 1]);
+        }
+      }
+    }
+    // dR^T and scale e^G dO^T as left operands of the state's cotangent
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      const int tok = n * 8 + 2 * t;
+      const float2 be = pair(beta + tok), eg = pair(eG + tok);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e = (i & 1) ? eg.y : eg.x, bb = (i & 1) ? be.y : be.x;
+        dy[n][i] *= -e * bb;
+        x[n][i] *= a.scale * e;
+      }
+    }
+    const float eC = eG[kC - 1];
+#pragma unroll
+    for (int n0 = 0; n0 < NT; n0 += NB) {
+      float acc[NB][4];
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) {
+        float y[4], hi[4], lo[4], hi2[4], lo2[4];
+        as_left(dy[ks], y);
+        split4(y, hi, lo);
+        as_left(x[ks], y);
+        split4(y, hi2, lo2);
+        float2 kk[NB], qq[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          const int at = (ks * 8 + 2 * t) * L::PK + kb + (n0 + n) * 8 + g;
+          kk[n] = make_float2(to_f<E>(K[at]), to_f<E>(K[at + L::PK]));
+          qq[n] = make_float2(to_f<E>(Q[at]), to_f<E>(Q[at + L::PK]));
+        }
+        mma_split<X, NB>(acc, hi, lo, kk);
+        mma_split<X, NB>(acc, hi2, lo2, qq);
+      }
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n0 + n][i] = fmaf(eC, s[n0 + n][i], acc[n][i]);
+    }
+    __syncthreads();
+  }
+  if (a.dinitial) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int kr = kb + n * 8 + 2 * t + (i & 1), d = d0 + (i >> 1) * 8;
+        if (kr < a.dk && d < a.dv) a.dinitial[((int64_t)bh * a.dk + kr) * a.dv + d] = s[n][i];
+      }
+  }
+}
+
+template <typename E, int DK, int WS>
+static int launch_scan_one(const Args& a, int groups, cudaStream_t st) {
+  const size_t bytes = BackScanLayout<E, DK>::bytes(groups, WS);
+  int rc = allow_smem(backward_scan_kernel<E, DK, WS>, bytes);
+  if (rc != BSX_OK) return rc;
+  const int per_head = (a.dv + 16 * groups - 1) / (16 * groups);
+  const unsigned grid = (unsigned)((int64_t)a.B * a.Hv * per_head);
+  backward_scan_kernel<E, DK, WS><<<grid, groups * WS * 32, bytes, st>>>(a, groups);
+  BSX_LAUNCH_CHECK("plastic backward_scan_kernel");
+  return BSX_OK;
+}
+
+template <typename E, int DK>
+static int launch_scan_typed(const Args& a, cudaStream_t st) {
+  const int64_t total = (int64_t)a.B * a.Hv * ((a.dv + 15) / 16);
+  const int most = (a.dv + 15) / 16;
+  const int sms = sm_count();
+  if (sms <= 0) return fail(BSX_ERR_CUDA, "no CUDA device");
+  const int ws = total <= 2 * (int64_t)sms ? 4 : (total <= 4 * (int64_t)sms ? 2 : 1);   // as in the forward pass
+  int groups = ws == 4 ? 1 : 4;
+  while (groups > most) groups >>= 1;
+  while (groups > 1 && BackScanLayout<E, DK>::bytes(groups, ws) > kMaxSmem) groups >>= 1;
+  if (ws == 4) return launch_scan_one<E, DK, 4>(a, groups, st);
+  if (ws == 2) return launch_scan_one<E, DK, 2>(a, groups, st);
+  return launch_scan_one<E, DK, 1>(a, groups, st);
+}
+
+// ------------------------------------------------------------------------------------------------ all chunks at once
+
+constexpr int kVB = 32;   // value columns of a block
+
+template <typename E, int DK>
+struct BackChunkLayout {
+  static constexpr int PK = DK + 8, PS = DK + 4, PY = kC + 4, PO = kVB + 8, PE = kC + 8;
+  static constexpr size_t tile = (size_t)kC * PK * sizeof(E);
+  // floats after the K and Q tiles
+  static constexpr int s0 = 0, ds = s0 + kVB * PS, u = ds + kVB * PS, dy = u + kVB * PY, dof = dy + kVB * PY,
+                       vf = dof + kC * PO, loop_end = vf + kC * PO;
+  static constexpr int e = 0, f = kC * PE, tail_end = 2 * kC * PE;       // reuse the block buffers
+  static constexpr int small = loop_end > tail_end ? loop_end : tail_end;
+  static constexpr int vecs = small, parts = vecs + kVec, end = parts + 20 * kC + 8;
+  static constexpr size_t bytes = 2 * tile + (size_t)end * sizeof(float);
+};
+
+template <typename E, int DK>
+__global__ void __launch_bounds__(256) backward_chunk_kernel(Args a) {
+  using L = BackChunkLayout<E, DK>;
+  constexpr bool X = IsExact<E>::value;
+  constexpr bool SHORT = IsShort<E>::value;
+  constexpr int NC4 = DK / 32;    // 8-wide column tiles of a warp in the (64, DK) products
+  extern __shared__ __align__(16) unsigned char smem[];
+  E* K = reinterpret_cast<E*>(smem);
+  E* Q = reinterpret_cast<E*>(smem + L::tile);
+  float* F = reinterpret_cast<float*>(smem + 2 * L::tile);
+  float* sS0 = F + L::s0;
+  float* sDS = F + L::ds;
+  float* sU = F + L::u;
+  float* sDY = F + L::dy;
+  float* sDO = F + L::dof;
+  float* sV = F + L::vf;
+  float* eG = F + L::vecs;
+  float* eD = eG + kC;
+  float* beta = eG + 2 * kC;
+  float* gHi = eG + 3 * kC;
+  float* gLo = eG + 4 * kC;
+  // parts: [0,4) row sums of dP P + dA A, [4,6) their column sums, [6,10) K.D1, [10,14) Q.Dq, [14,18) K.D3,
+  //        18 dY.V, 19 row sums of dA (A/beta) by column quarter come in [0,4) of a second use
+  float* parts = F + L::parts;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int wr = warp & 1, wc = warp >> 1;     // rows 32 wr .. + 31; columns by quarter wc
+  const int chunk = blockIdx.x % a.NC;
+  const int bh = blockIdx.x / a.NC, b = bh / a.Hv, h = bh - b * a.Hv, hk = h / (a.Hv / a.Hk);
+  const int len = row_length(a, b);
+  const int64_t t0 = (int64_t)chunk * kC;
+  if (t0 >= len) return;
+  const int rows = (int)min((int64_t)kC, len - t0);
+  const int64_t ci = (int64_t)bh * a.NC + chunk;
+
+  stage(K, L::PK, static_cast<const E*>(a.k) + b * a.ks[0] + t0 * a.ks[1] + hk * a.ks[2], a.ks[1], rows, a.dk, DK,
+        a.vec_qk, tid, 256);
+  stage(Q, L::PK, static_cast<const E*>(a.q) + b * a.qs[0] + t0 * a.qs[1] + hk * a.qs[2], a.qs[1], rows, a.dk, DK,
+        a.vec_qk, tid, 256);
+  for (int i = tid; i < kVec / 4; i += 256) cp16(eG + i * 4, a.vec + ci * kVec + i * 4, true);
+  cp_commit();
+
+  float d1[2][NC4][4], dqa[2][NC4][4], d3[2][NC4][4], dp[2][2][4], da[2][2][4];
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+#pragma unroll
+    for (int n = 0; n < NC4; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) d1[m][n][i] = dqa[m][n][i] = d3[m][n][i] = 0.f;
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) dp[m][n][i] = da[m][n][i] = 0.f;
+  }
+  float ss = 0.f;     // <S0, dS>
+  float yv = 0.f;     // dY.V of token tid >> 2, columns tid & 3 mod 4
+  const int64_t os = (int64_t)a.Hv * a.dv;
+  const E* dop = static_cast<const E*>(a.dout) + ((int64_t)b * a.T + t0) * os + (int64_t)h * a.dv;
+  const E* vp = static_cast<const E*>(a.v) + b * a.vs[0] + t0 * a.vs[1] + h * a.vs[2];
+  const float* gS = a.Sn + ci * a.dv * DK;
+  const float* gDS = a.dS + ci * a.dv * DK;
+  const float* gU = a.U + ci * a.dv * kC;
+  const float* gY = a.dY + ci * a.dv * kC;
+
+  for (int v0 = 0; v0 < a.dv; v0 += kVB) {
+    const int nv = min(kVB, a.dv - v0);
+    __syncthreads();
+    for (int i = tid; i < kVB * DK / 4; i += 256) {
+      const int r = i / (DK / 4), c = (i - r * (DK / 4)) * 4;
+      const bool ok = r < nv;
+      const int64_t at = ok ? (int64_t)(v0 + r) * DK + c : 0;
+      cp16(sS0 + r * L::PS + c, gS + at, ok);
+      cp16(sDS + r * L::PS + c, gDS + at, ok);
+    }
+    for (int i = tid; i < kVB * kC / 4; i += 256) {
+      const int r = i / (kC / 4), c = (i - r * (kC / 4)) * 4;
+      const bool ok = r < nv;
+      const int64_t at = ok ? (int64_t)(v0 + r) * kC + c : 0;
+      cp16(sU + r * L::PY + c, gU + at, ok);
+      cp16(sDY + r * L::PY + c, gY + at, ok);
+    }
+    cp_commit();
+    for (int i = tid; i < kC * kVB; i += 256) {
+      const int r = i / kVB, c = i - r * kVB;
+      const bool ok = r < rows && c < nv;
+      sDO[r * L::PO + c] = ok ? to_f<E>(dop[r * os + v0 + c]) : 0.f;
+      sV[r * L::PO + c] = ok ? to_f<E>(vp[r * a.vs[1] + v0 + c]) : 0.f;
+    }
+    cp_wait<0>();
+    __syncthreads();
+    // <S0, dS> and dY.V in 32-bit arithmetic
+    for (int i = tid; i < kVB * DK; i += 256) {
+      const int r = i / DK, c = i - r * DK;
+      ss = fmaf(sS0[r * L::PS + c], sDS[r * L::PS + c], ss);
+    }
+    {
+      const int tok = tid >> 2;
+#pragma unroll
+      for (int c = 0; c < kVB / 4; ++c) {
+        const int v = c * 4 + (tid & 3);
+        yv = fmaf(sDY[v * L::PY + tok], sV[tok * L::PO + v], yv);
+      }
+    }
+#pragma unroll
+    for (int ks = 0; ks < kVB / 8; ++ks) {
+      const int vr = ks * 8 + 2 * t;
+      float oh[2][4], ol[2][4], yh[2][4], yl[2][4], uh[2][4], ul[2][4];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const int i = wr * 32 + m * 16 + g;
+        const float2 p0 = pair(sDO + i * L::PO + vr), p1 = pair(sDO + (i + 8) * L::PO + vr);
+        const float ao[4] = {p0.x, p1.x, p0.y, p1.y};
+        if (X) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) oh[m][e] = ao[e];
+        } else {
+          split4(ao, oh[m], ol[m]);
+        }
+        const float* y = sDY + vr * L::PY + i;
+        const float ay[4] = {y[0], y[8], y[L::PY], y[L::PY + 8]};
+        split4(ay, yh[m], yl[m]);
+        const float* u = sU + vr * L::PY + i;
+        const float au[4] = {u[0], u[8], u[L::PY], u[L::PY + 8]};
+        split4(au, uh[m], ul[m]);
+      }
+#pragma unroll
+      for (int n = 0; n < NC4; ++n) {
+        const int col = wc * (DK / 4) + n * 8 + g;
+        float h0, l0, h1, l1;
+        split(sS0[vr * L::PS + col], h0, l0);
+        split(sS0[(vr + 1) * L::PS + col], h1, l1);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          mma(d1[m][n], yl[m], h0, h1);
+          mma(dqa[m][n], oh[m], l0, l1);
+          mma(d1[m][n], yh[m], l0, l1);
+          if (!X) mma(dqa[m][n], ol[m], h0, h1);
+          mma(d1[m][n], yh[m], h0, h1);
+          mma(dqa[m][n], oh[m], h0, h1);
+        }
+        split(sDS[vr * L::PS + col], h0, l0);
+        split(sDS[(vr + 1) * L::PS + col], h1, l1);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          mma(d3[m][n], ul[m], h0, h1);
+          mma(d3[m][n], uh[m], l0, l1);
+          mma(d3[m][n], uh[m], h0, h1);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int col = wc * 16 + n * 8 + g;
+        float h0, l0, h1, l1;
+        split(sU[vr * L::PY + col], h0, l0);
+        split(sU[(vr + 1) * L::PY + col], h1, l1);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          mma(dp[m][n], oh[m], l0, l1);
+          if (!X) mma(dp[m][n], ol[m], h0, h1);
+          mma(dp[m][n], oh[m], h0, h1);
+          mma(da[m][n], yl[m], h0, h1);
+          mma(da[m][n], yh[m], l0, l1);
+          mma(da[m][n], yh[m], h0, h1);
+        }
+      }
+    }
+  }
+  __syncthreads();
+
+  // dot products over the key rows
+  float pk1[4], pkq[4], pk3[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {   // row wr * 32 + (r >> 1) * 16 + (r & 1) * 8 + g
+    const int i = wr * 32 + (r >> 1) * 16 + (r & 1) * 8 + g;
+    float x1 = 0.f, xq = 0.f, x3 = 0.f;
+#pragma unroll
+    for (int n = 0; n < NC4; ++n) {
+      const int col = wc * (DK / 4) + n * 8 + 2 * t;
+      const float2 kk = pair(K + i * L::PK + col), qq = pair(Q + i * L::PK + col);
+      const int e = 2 * (r & 1);
+      x1 += kk.x * d1[r >> 1][n][e] + kk.y * d1[r >> 1][n][e + 1];
+      xq += qq.x * dqa[r >> 1][n][e] + qq.y * dqa[r >> 1][n][e + 1];
+      x3 += kk.x * d3[r >> 1][n][e] + kk.y * d3[r >> 1][n][e + 1];
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      x1 += __shfl_xor_sync(0xffffffffu, x1, o);
+      xq += __shfl_xor_sync(0xffffffffu, xq, o);
+      x3 += __shfl_xor_sync(0xffffffffu, x3, o);
+    }
+    pk1[r] = x1; pkq[r] = xq; pk3[r] = x3;
+    if (t == 0) {
+      parts[(6 + wc) * kC + i] = pk1[r];
+      parts[(10 + wc) * kC + i] = pkq[r];
+      parts[(14 + wc) * kC + i] = pk3[r];
+    }
+  }
+  yv += __shfl_xor_sync(0xffffffffu, yv, 1);
+  yv += __shfl_xor_sync(0xffffffffu, yv, 2);
+  if ((tid & 3) == 0) parts[18 * kC + (tid >> 2)] = yv;
+  ss = warp_sum(ss);
+  if (lane == 0) parts[20 * kC + warp] = ss;
+
+  // E, F and the sums of dP P + dA A, dA (A/beta)
+  float* sE = F + L::e;
+  float* sF = F + L::f;
+  const float* Pm = a.Pm + ci * kC * kC;
+  const float* Bm = a.Bm + ci * kC * kC;
+  float cs[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+  float bsum[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int i = wr * 32 + (r >> 1) * 16 + (r & 1) * 8 + g;
+    float rs = 0.f, bsr = 0.f;
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int j = wc * 16 + n * 8 + 2 * t + e;
+        float ev = 0.f, fv = 0.f;
+        if (j <= i) {
+          const float gam = expf((gHi[i] - gHi[j]) + (gLo[i] - gLo[j]));
+          const float dpv = dp[r >> 1][n][2 * (r & 1) + e];
+          float m = dpv * Pm[i * kC + j];
+          ev = a.scale * gam * dpv;
+          if (j < i) {
+            const float dav = -da[r >> 1][n][2 * (r & 1) + e];
+            const float nb = dav * Bm[i * kC + j];
+            bsr += nb;
+            m = fmaf(beta[i], nb, m);
+            fv = beta[i] * gam * dav;
+          }
+          rs += m;
+          cs[n][e] += m;
+        }
+        sE[i * L::PE + j] = ev;
+        sF[i * L::PE + j] = fv;
+      }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      rs += __shfl_xor_sync(0xffffffffu, rs, o);
+      bsr += __shfl_xor_sync(0xffffffffu, bsr, o);
+    }
+    if (t == 0) parts[wc * kC + i] = rs;
+    bsum[r] = bsr;
+  }
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float x = cs[n][e];
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+      if (g == 0) parts[(4 + wr) * kC + wc * 16 + n * 8 + 2 * t + e] = x;
+    }
+  __syncthreads();
+
+  // gates: thread i < 64 has token i
+  float dG = 0.f, dbe = 0.f, tailC = 0.f;
+  if (tid < kC) {
+    const int i = tid;
+    float c1 = 0.f, cq = 0.f, c3 = 0.f, rs = 0.f;
+    for (int p = 0; p < 4; ++p) {
+      c1 += parts[(6 + p) * kC + i];
+      cq += parts[(10 + p) * kC + i];
+      c3 += parts[(14 + p) * kC + i];
+      rs += parts[p * kC + i];
+    }
+    const float cc = parts[4 * kC + i] + parts[5 * kC + i];
+    const float L3 = eD[i] * c3;
+    dbe = parts[18 * kC + i] - eG[i] * c1;
+    dG = (rs - cc) - beta[i] * eG[i] * c1 + a.scale * eG[i] * cq - L3;
+    tailC = L3;
+  }
+  __syncthreads();
+  if (t == 0) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) parts[wc * kC + wr * 32 + (r >> 1) * 16 + (r & 1) * 8 + g] = bsum[r];
+  }
+  if (tid < kC) {
+    parts[4 * kC + tid] = dG;
+    parts[5 * kC + tid] = tailC;
+  }
+  __syncthreads();
+  if (tid < kC) {
+    const int i = tid;
+    dbe += (parts[i] + parts[kC + i]) + (parts[2 * kC + i] + parts[3 * kC + i]);
+    if (i < rows) a.dbeta[((int64_t)b * a.T + t0 + i) * a.Hv + h] = dbe;
+  }
+  if (warp == 2) {   // dg: sums of dG from the end; the chunk's last G takes the tail terms
+    const float* sdG = parts + 4 * kC;
+    const float* sTail = parts + 5 * kC;
+    float x0 = sdG[2 * lane], x1 = sdG[2 * lane + 1];
+    float tail = warp_sum(sTail[2 * lane] + sTail[2 * lane + 1]);
+    float in = 0.f;
+    for (int p = 0; p < 8; ++p) in += parts[20 * kC + p];
+    tail += eG[kC - 1] * in;
+    float s = x0 + x1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const float y = __shfl_down_sync(0xffffffffu, s, o);
+      if (lane + o < 32) s += y;
+    }
+    const float e0 = s + tail, e1 = (s - x0) + tail;
+    if (2 * lane < rows) a.dg[((int64_t)b * a.T + t0 + 2 * lane) * a.Hv + h] = e0;
+    if (2 * lane + 1 < rows) a.dg[((int64_t)b * a.T + t0 + 2 * lane + 1) * a.Hv + h] = e1;
+  }
+
+  // dQ and dK on top of the parts that came through the state
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int n = 0; n < NC4; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int tok = wr * 32 + m * 16 + g + 8 * (i >> 1);
+        dqa[m][n][i] *= a.scale * eG[tok];
+        d1[m][n][i] = fmaf(-beta[tok] * eG[tok], d1[m][n][i], eD[tok] * d3[m][n][i]);
+      }
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks) {
+    float eh[2][4], el[2][4], th[2][4], tl[2][4], fh[2][4], fl[2][4];
+    const int c0 = ks * 8 + 2 * t;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const int i = wr * 32 + m * 16 + g;
+      const float2 p0 = pair(sE + i * L::PE + c0), p1 = pair(sE + (i + 8) * L::PE + c0);
+      const float ae[4] = {p0.x, p1.x, p0.y, p1.y};
+      const float* et = sE + c0 * L::PE + i;
+      const float at[4] = {et[0], et[8], et[L::PE], et[L::PE + 8]};
+      const float2 f0 = pair(sF + i * L::PE + c0), f1 = pair(sF + (i + 8) * L::PE + c0);
+      const float* ft = sF + c0 * L::PE + i;
+      const float af[4] = {f0.x + ft[0], f1.x + ft[8], f0.y + ft[L::PE], f1.y + ft[L::PE + 8]};
+      if (SHORT) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          eh[m][e] = tf32(ae[e]);
+          th[m][e] = tf32(at[e]);
+          fh[m][e] = tf32(af[e]);
+        }
+      } else {
+        split4(ae, eh[m], el[m]);
+        split4(at, th[m], tl[m]);
+        split4(af, fh[m], fl[m]);
+      }
+    }
+    float2 kk[NC4], qq[NC4];
+#pragma unroll
+    for (int n = 0; n < NC4; ++n) {
+      const int at = c0 * L::PK + wc * (DK / 4) + n * 8 + g;
+      kk[n] = make_float2(to_f<E>(K[at]), to_f<E>(K[at + L::PK]));
+      qq[n] = make_float2(to_f<E>(Q[at]), to_f<E>(Q[at + L::PK]));
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      if (SHORT) {
+#pragma unroll
+        for (int n = 0; n < NC4; ++n) mma(dqa[m][n], eh[m], kk[n].x, kk[n].y);
+#pragma unroll
+        for (int n = 0; n < NC4; ++n) mma(d1[m][n], th[m], qq[n].x, qq[n].y);
+#pragma unroll
+        for (int n = 0; n < NC4; ++n) mma(d1[m][n], fh[m], kk[n].x, kk[n].y);
+      } else {
+        mma_split<X, NC4>(dqa[m], eh[m], el[m], kk);
+        mma_split<X, NC4>(d1[m], th[m], tl[m], qq);
+        mma_split<X, NC4>(d1[m], fh[m], fl[m], kk);
+      }
+    }
+  }
+  const bool shared = a.Hk != a.Hv;
+  const int heads = shared ? a.Hv : a.Hk, ho = shared ? h : hk;
+  const int64_t ob = (((int64_t)b * a.T + t0) * heads + ho) * a.dk;
+  const int64_t ots = (int64_t)heads * a.dk;
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int n = 0; n < NC4; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int tok = wr * 32 + m * 16 + g + 8 * (i >> 1), col = wc * (DK / 4) + n * 8 + 2 * t + (i & 1);
+        if (tok >= rows || col >= a.dk) continue;
+        const int64_t at = ob + tok * ots + col;
+        if (shared) {
+          a.dq32[at] = dqa[m][n][i];
+          a.dk32[at] = d1[m][n][i];
+        } else {
+          static_cast<E*>(a.dq)[at] = from_f<E>(dqa[m][n][i]);
+          static_cast<E*>(a.dk_)[at] = from_f<E>(d1[m][n][i]);
+        }
+      }
+}
+
+// Gradients of keys and queries that several value heads share: 32-bit sums in head order.
+template <typename E>
+__global__ void __launch_bounds__(256) head_sum_kernel(Args a) {
+  const int group = a.Hv / a.Hk;
+  const int64_t n = (int64_t)a.B * a.T * a.Hk * a.dk;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / a.dk, tb = row / a.Hk, tok = tb % a.T;
+    const int c = (int)(i - row * a.dk), b = (int)(tb / a.T);
+    float xq = 0.f, xk = 0.f;
+    if (tok < row_length(a, b)) {
+      const int64_t at = row * group * a.dk + c;
+      for (int p = 0; p < group; ++p) {
+        xq += a.dq32[at + (int64_t)p * a.dk];
+        xk += a.dk32[at + (int64_t)p * a.dk];
+      }
+    }
+    static_cast<E*>(a.dq)[i] = from_f<E>(xq);
+    static_cast<E*>(a.dk_)[i] = from_f<E>(xk);
+  }
+}
+
+template <typename E, int DK>
+static int launch_chunks_typed(const Args& a, cudaStream_t st) {
+  const size_t bytes = BackChunkLayout<E, DK>::bytes;
+  int rc = allow_smem(backward_chunk_kernel<E, DK>, bytes);
+  if (rc != BSX_OK) return rc;
+  backward_chunk_kernel<E, DK><<<(unsigned)((int64_t)a.B * a.Hv * a.NC), 256, bytes, st>>>(a);
+  BSX_LAUNCH_CHECK("plastic backward_chunk_kernel");
+  if (a.Hk != a.Hv) {
+    const int64_t n = (int64_t)a.B * a.T * a.Hk * a.dk;
+    const int64_t want = (n + 255) / 256, most = 16ll * sm_count();
+    head_sum_kernel<E><<<(unsigned)(want < most ? want : most), 256, 0, st>>>(a);
+    BSX_LAUNCH_CHECK("plastic head_sum_kernel");
+  }
+  return BSX_OK;
+}
+
+int launch_backward_scan(const Args& a, int dtype, cudaStream_t st) {
+  const bool narrow = a.dk <= 64;
+  if (dtype == BSX_T_F32) return narrow ? launch_scan_typed<float, 64>(a, st) : launch_scan_typed<float, 128>(a, st);
+  if (dtype == BSX_T_BF16)
+    return narrow ? launch_scan_typed<__nv_bfloat16, 64>(a, st) : launch_scan_typed<__nv_bfloat16, 128>(a, st);
+  return narrow ? launch_scan_typed<__half, 64>(a, st) : launch_scan_typed<__half, 128>(a, st);
+}
+
+int launch_backward_chunks(const Args& a, int dtype, cudaStream_t st) {
+  const bool narrow = a.dk <= 64;
+  if (dtype == BSX_T_F32) return narrow ? launch_chunks_typed<float, 64>(a, st) : launch_chunks_typed<float, 128>(a, st);
+  if (dtype == BSX_T_BF16)
+    return narrow ? launch_chunks_typed<__nv_bfloat16, 64>(a, st) : launch_chunks_typed<__nv_bfloat16, 128>(a, st);
+  return narrow ? launch_chunks_typed<__half, 64>(a, st) : launch_chunks_typed<__half, 128>(a, st);
+}
+
+}  // namespace plastic
+}  // namespace bsx

@@ -1,0 +1,212 @@
+// Gated delta rule: what a chunk needs that does not depend on the state — T, P and the decay vectors — for all
+// chunks at once, one block of four warps per (row, head, chunk).
+//
+// K K^T and Q K^T are 64x64xdk products (only the tiles on and below the diagonal); T = (I + A)^{-1} is built by
+// substitution: the four 16x16 diagonal blocks by columns (one lane each), then
+// T_ij = -T_ii sum_l A_il T_lj by block distance, in 32-bit arithmetic.  (A power series would need fewer steps but
+// loses all digits when the keys of a chunk are alike.)  The sums of g are taken in 64 bits and kept as two floats, so
+// that a strong decay (g is cut at -128, where e^g is 0 in 32 bits) leaves the differences behind it exact.
+#include "plastic.cuh"
+
+namespace bsx {
+namespace plastic {
+
+template <typename E, int DK>
+struct PrepLayout {
+  static constexpr int PK = sizeof(E) == 2 ? DK + 8 : DK + 8;  // pair loads of 8 rows hit distinct banks
+  static constexpr size_t tile = (size_t)kC * PK * sizeof(E);
+  static constexpr int PA = kC + 1;
+  static constexpr size_t bytes = 2 * tile + sizeof(float) * (2 * kC * PA + 3 * 256 + 4 * kC) + 16;
+};
+
+template <typename E, int DK, bool BACK>
+__global__ void __launch_bounds__(128) prepare_kernel(Args a) {
+  using L = PrepLayout<E, DK>;
+  extern __shared__ __align__(16) unsigned char smem[];
+  E* sk = reinterpret_cast<E*>(smem);
+  E* sq = reinterpret_cast<E*>(smem + L::tile);
+  float* sA = reinterpret_cast<float*>(smem + 2 * L::tile);
+  float* sT = sA + kC * L::PA;
+  float* sW = sT + kC * L::PA;      // 3 x 16 x 16
+  float* sHi = sW + 3 * 256;
+  float* sLo = sHi + kC;
+  float* sBeta = sLo + kC;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int chunk = blockIdx.x % a.NC;
+  const int bh = blockIdx.x / a.NC, b = bh / a.Hv, h = bh - b * a.Hv, hk = h / (a.Hv / a.Hk);
+  const int len = row_length(a, b);
+  const int64_t t0 = (int64_t)chunk * kC;
+  if (t0 >= len) return;
+  const int rows = (int)min((int64_t)kC, len - t0);
+  const int64_t ci = (int64_t)bh * a.NC + chunk;
+
+  const E* kp = static_cast<const E*>(a.k) + b * a.ks[0] + t0 * a.ks[1] + hk * a.ks[2];
+  const E* qp = static_cast<const E*>(a.q) + b * a.qs[0] + t0 * a.qs[1] + hk * a.qs[2];
+  stage(sk, L::PK, kp, a.ks[1], rows, a.dk, DK, a.vec_qk, tid, 128);
+  stage(sq, L::PK, qp, a.qs[1], rows, a.dk, DK, a.vec_qk, tid, 128);
+  cp_commit();
+  if (warp == 0) {  // sums of g: two tokens a lane, then across the lanes
+    const float* gp = a.g + b * a.gs[0] + t0 * a.gs[1] + h * a.gs[2];
+    const float* bp = a.beta + b * a.bs[0] + t0 * a.bs[1] + h * a.bs[2];
+    double x0 = 0, x1 = 0;
+    float b0 = 0.f, b1 = 0.f;
+    if (2 * lane < rows) {
+      const float v = gp[(2 * lane) * a.gs[1]];
+      x0 = v < -128.f ? -128.f : v;
+      b0 = bp[(2 * lane) * a.bs[1]];
+    }
+    if (2 * lane + 1 < rows) {
+      const float v = gp[(2 * lane + 1) * a.gs[1]];
+      x1 = v < -128.f ? -128.f : v;
+      b1 = bp[(2 * lane + 1) * a.bs[1]];
+    }
+    double s = x0 + x1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double y = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += y;
+    }
+    const double G1 = s, G0 = s - x1, GC = __shfl_sync(0xffffffffu, s, 31);
+    // s - x1 is not the sum in order, but within 2^-52 of it
+    float* vec = a.vec + ci * kVec;
+    const float h0 = (float)G0, h1 = (float)G1;
+    const float l0 = (float)(G0 - h0), l1 = (float)(G1 - h1);
+    sHi[2 * lane] = h0; sHi[2 * lane + 1] = h1;
+    sLo[2 * lane] = l0; sLo[2 * lane + 1] = l1;
+    sBeta[2 * lane] = b0; sBeta[2 * lane + 1] = b1;
+    *reinterpret_cast<float2*>(vec + 2 * lane) = make_float2(expf((float)G0), expf((float)G1));
+    *reinterpret_cast<float2*>(vec + kC + 2 * lane) = make_float2(expf((float)(GC - G0)), expf((float)(GC - G1)));
+    *reinterpret_cast<float2*>(vec + 2 * kC + 2 * lane) = make_float2(b0, b1);
+    *reinterpret_cast<float2*>(vec + 3 * kC + 2 * lane) = make_float2(h0, h1);
+    *reinterpret_cast<float2*>(vec + 4 * kC + 2 * lane) = make_float2(l0, l1);
+  }
+  cp_wait<0>();
+  __syncthreads();
+
+  // rows 16 * warp .. + 15 of K K^T and Q K^T, tiles on and below the diagonal
+  float kk[8][4], qk[8][4];
+#pragma unroll
+  for (int n = 0; n < 8; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) kk[n][i] = qk[n][i] = 0.f;
+  const int r0 = warp * 16 + g;
+  for (int ks = 0; ks < DK / 8; ++ks) {
+    const int c = ks * 8 + 2 * t;
+    const float2 k0 = pair(sk + r0 * L::PK + c), k1 = pair(sk + (r0 + 8) * L::PK + c);
+    const float2 q0 = pair(sq + r0 * L::PK + c), q1 = pair(sq + (r0 + 8) * L::PK + c);
+    float ak[4] = {k0.x, k1.x, k0.y, k1.y}, aq[4] = {q0.x, q1.x, q0.y, q1.y};
+    float akl[4], aql[4], akh[4], aqh[4];
+    if (!IsExact<E>::value) {
+      split4(ak, akh, akl);
+      split4(aq, aqh, aql);
+    }
+#pragma unroll
+    for (int n0 = 0; n0 < 8; n0 += 2) {
+      if (n0 > 2 * warp) break;
+      float2 bb[2];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) bb[n] = pair(sk + ((n0 + n) * 8 + g) * L::PK + c);
+      if (IsExact<E>::value) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          mma(kk[n0 + n], ak, bb[n].x, bb[n].y);
+          mma(qk[n0 + n], aq, bb[n].x, bb[n].y);
+        }
+      } else {
+        mma_split<false, 2>(kk + n0, akh, akl, bb);
+        mma_split<false, 2>(qk + n0, aqh, aql, bb);
+      }
+    }
+  }
+  float* Pm = a.Pm + ci * (kC * kC);
+  float* Bm = BACK ? a.Bm + ci * (kC * kC) : nullptr;
+#pragma unroll
+  for (int n = 0; n < 8; ++n) {
+    if (n > 2 * warp + 1) break;
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const int i = r0 + 8 * hf, j = n * 8 + 2 * t;
+      float p[2], m[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float gam = j + e <= i ? expf((sHi[i] - sHi[j + e]) + (sLo[i] - sLo[j + e])) : 0.f;
+        p[e] = j + e <= i ? a.scale * gam * qk[n][2 * hf + e] : 0.f;
+        m[e] = j + e < i ? gam * kk[n][2 * hf + e] : 0.f;
+        sA[i * L::PA + j + e] = sBeta[i] * m[e];
+      }
+      *reinterpret_cast<float2*>(Pm + i * kC + j) = make_float2(p[0], p[1]);
+      if (BACK) *reinterpret_cast<float2*>(Bm + i * kC + j) = make_float2(m[0], m[1]);
+    }
+  }
+  __syncthreads();
+
+  // diagonal blocks of T: lane j solves column j of block `warp`
+  if (lane < 16) {
+    float x[16];
+    const float* Ad = sA + (16 * warp) * L::PA + 16 * warp;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float v = i == lane ? 1.f : 0.f;
+#pragma unroll
+      for (int l = 0; l < 16; ++l)
+        if (l < i) v = fmaf(-Ad[i * L::PA + l], x[l], v);
+      x[i] = v;
+      sT[(16 * warp + i) * L::PA + 16 * warp + lane] = v;
+    }
+  }
+  __syncthreads();
+  for (int d = 1; d < 4; ++d) {
+    const int n = (4 - d) * 256;
+    for (int e = tid; e < n; e += 128) {
+      const int blk = e >> 8, r = (e >> 4) & 15, c = e & 15, j = blk, i = blk + d;
+      float v = 0.f;
+      for (int l = j * 16; l < i * 16; ++l) v = fmaf(sA[(i * 16 + r) * L::PA + l], sT[l * L::PA + j * 16 + c], v);
+      sW[e] = v;
+    }
+    __syncthreads();
+    for (int e = tid; e < n; e += 128) {
+      const int blk = e >> 8, r = (e >> 4) & 15, c = e & 15, j = blk, i = blk + d;
+      float v = 0.f;
+#pragma unroll
+      for (int l = 0; l < 16; ++l) v = fmaf(-sT[(i * 16 + r) * L::PA + i * 16 + l], sW[blk * 256 + l * 16 + c], v);
+      sT[(i * 16 + r) * L::PA + j * 16 + c] = v;
+    }
+    __syncthreads();
+  }
+  float* Tm = a.Tm + ci * (kC * kC);
+  for (int e = tid; e < kC * kC; e += 128) {
+    const int r = e >> 6, c = e & 63;
+    if (c < ((r >> 4) + 1) * 16) Tm[e] = sT[r * L::PA + c];
+  }
+}
+
+template <typename E, int DK>
+static int launch_typed(const Args& a, bool backward, cudaStream_t st) {
+  const size_t bytes = PrepLayout<E, DK>::bytes;
+  const unsigned grid = (unsigned)((int64_t)a.B * a.Hv * a.NC);
+  int rc;
+  if (backward) {
+    if ((rc = allow_smem(prepare_kernel<E, DK, true>, bytes)) != BSX_OK) return rc;
+    prepare_kernel<E, DK, true><<<grid, 128, bytes, st>>>(a);
+  } else {
+    if ((rc = allow_smem(prepare_kernel<E, DK, false>, bytes)) != BSX_OK) return rc;
+    prepare_kernel<E, DK, false><<<grid, 128, bytes, st>>>(a);
+  }
+  BSX_LAUNCH_CHECK("plastic prepare_kernel");
+  return BSX_OK;
+}
+
+template <typename E>
+static int launch_width(const Args& a, bool backward, cudaStream_t st) {
+  return a.dk <= 64 ? launch_typed<E, 64>(a, backward, st) : launch_typed<E, 128>(a, backward, st);
+}
+
+int launch_prepare(const Args& a, int dtype, bool backward, cudaStream_t st) {
+  if (dtype == BSX_T_F32) return launch_width<float>(a, backward, st);
+  if (dtype == BSX_T_BF16) return launch_width<__nv_bfloat16>(a, backward, st);
+  return launch_width<__half>(a, backward, st);
+}
+
+}  // namespace plastic
+}  // namespace bsx

@@ -1,0 +1,222 @@
+"""Plastic synapses: weight matrices that learn while they are used.
+
+The gated delta rule keeps a synaptic matrix ``S`` of shape ``(dk, dv)`` per batch row and value
+head.  Every token (time step) first lets the matrix decay, then corrects its answer to the key
+towards the value (an error-correcting Hebbian update), then answers the query::
+
+    u_t = beta_t (v_t - e^{g_t} S_{t-1}^T k_t)
+    S_t = e^{g_t} S_{t-1} + k_t u_t^T
+    o_t = scale S_t^T q_t
+
+``delta_rule`` runs whole sequences (chunked over 64 tokens on the tensor cores, differentiable),
+``delta_rule_step`` one token with the state updated in place.  States are float32; sums and
+everything the state depends on are held to 32-bit accuracy also for 16-bit inputs.  Keys should
+have a norm of at most about 1 and ``beta`` lie in [0, 1] (the rule diverges where
+``beta |k|^2 > 2``); ``g`` is at most 0, and ``-inf`` drops the state.  Kernels:
+``csrc/plastic*.cu``.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import BsxDelta, check, lib, ptr
+from .event import _require_cuda
+
+__all__ = ['delta_rule', 'delta_rule_step']
+
+_TYPES = {torch.float32: _lib.T_F32, torch.bfloat16: _lib.T_BF16, torch.float16: _lib.T_F16}
+
+# Sequences of at most this many tokens go token by token (one launch, the state read and written
+# once) instead of by chunks.
+RECURRENT_TOKENS = 16
+
+
+def _dense_rows(t: torch.Tensor) -> torch.Tensor:
+    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _strides(t: torch.Tensor):
+    # the stride of a dimension of one entry says nothing and must not spoil the alignment rule
+    return tuple(0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3]))
+
+
+def _describe(q, k, v, g, beta, initial, lengths, scale) -> BsxDelta:
+    d = BsxDelta()
+    d.batch, d.tokens, d.k_heads, d.dk = q.shape
+    d.v_heads, d.dv = v.shape[2:]
+    d.dtype, d.scale = _TYPES[q.dtype], scale
+    d.q, d.k, d.v, d.g, d.beta = q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr()
+    d.initial, d.lengths = ptr(initial), ptr(lengths)
+    d.q_stride[:], d.k_stride[:], d.v_stride[:] = _strides(q), _strides(k), _strides(v)
+    d.g_stride[:], d.beta_stride[:] = _strides(g), _strides(beta)
+    return d
+
+
+def _stream(t: torch.Tensor) -> int:
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+class _DeltaRule(torch.autograd.Function):
+
+    @staticmethod
+    def forward(q, k, v, g, beta, initial, lengths, scale):
+        B, T, _, dk = q.shape
+        Hv, dv = v.shape[2:]
+        # tokens past a row's length are not written by the kernels
+        o = (torch.empty if lengths is None else torch.zeros)((B, T, Hv, dv), dtype=v.dtype, device=v.device)
+        state = torch.empty((B, Hv, dk, dv), dtype=torch.float32, device=v.device)
+        with torch.cuda.device(v.device):
+            d = _describe(q, k, v, g, beta, initial, lengths, scale)
+            if T <= RECURRENT_TOKENS:
+                check(lib().bsx_delta_recurrent(C.byref(d), ptr(o), ptr(state), _stream(v)))
+            else:
+                n = lib().bsx_delta_workspace_bytes(C.byref(d))
+                ws = torch.empty(n, dtype=torch.uint8, device=v.device)
+                check(lib().bsx_delta_forward(C.byref(d), ptr(o), ptr(state), ptr(ws), n, _stream(v)))
+        return o, state
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        q, k, v, g, beta, initial, lengths, scale = inputs
+        ctx.scale = scale
+        ctx.save_for_backward(q, k, v, g, beta, initial, lengths)
+        ctx.set_materialize_grads(False)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do, dstate):
+        if do is None and dstate is None:
+            return (None,) * 8
+        q, k, v, g, beta, initial, lengths = ctx.saved_tensors
+        make = torch.empty if lengths is None else torch.zeros
+        if do is None:
+            do = torch.zeros((*v.shape,), dtype=v.dtype, device=v.device)
+        do = do.contiguous()
+        dstate = None if dstate is None else dstate.contiguous()
+        dq, dk, dv = (make(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dg, dbeta = (make(t.shape, dtype=torch.float32, device=t.device) for t in (g, beta))
+        dinitial = torch.empty_like(initial) if ctx.needs_input_grad[5] else None
+        with torch.cuda.device(v.device):
+            d = _describe(q, k, v, g, beta, initial, lengths, ctx.scale)
+            n = lib().bsx_delta_backward_workspace_bytes(C.byref(d))
+            ws = torch.empty(max(n, 1), dtype=torch.uint8, device=v.device)
+            check(lib().bsx_delta_backward(C.byref(d), ptr(do), ptr(dstate), ptr(dq), ptr(dk), ptr(dv), ptr(dg),
+                                           ptr(dbeta), ptr(dinitial), ptr(ws), n, _stream(v)))
+        return dq, dk, dv, dg, dbeta, dinitial, None, None
+
+
+def _check(q, k, v, g, beta, state, lead: int):
+    """Refuses what the kernels do not take; ``lead`` is the number of dimensions before the heads."""
+    for name, t, dims in (('q', q, lead + 2), ('k', k, lead + 2), ('v', v, lead + 2), ('g', g, lead + 1),
+                          ('beta', beta, lead + 1)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f'{name} must be a tensor')
+        _require_cuda(t, name)
+        if t.dim() != dims:
+            raise ValueError(f'{name} has {t.dim()} dimensions, expected {dims}')
+        if t.device != q.device:
+            raise ValueError(f'{name} is on {t.device}, q on {q.device}')
+    if q.dtype not in _TYPES:
+        raise TypeError(f'q, k and v must be float32, bfloat16 or float16, got {q.dtype}')
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f'q, k and v must have one type, got {q.dtype}, {k.dtype} and {v.dtype}')
+    for name, t in (('g', g), ('beta', beta)):
+        if not t.dtype.is_floating_point:
+            raise TypeError(f'{name} must be floating point, got {t.dtype}')
+    if k.shape != q.shape:
+        raise ValueError(f'q {tuple(q.shape)} and k {tuple(k.shape)} differ in shape')
+    if v.shape[:lead] != q.shape[:lead]:
+        raise ValueError(f'v {tuple(v.shape)} does not go with q {tuple(q.shape)}')
+    if g.shape != v.shape[:-1] or beta.shape != v.shape[:-1]:
+        raise ValueError(f'g {tuple(g.shape)} and beta {tuple(beta.shape)} must have the shape {tuple(v.shape[:-1])}')
+    hk, dk = q.shape[-2:]
+    hv, dv = v.shape[-2:]
+    if hk < 1 or hv < 1 or hv % hk != 0:
+        raise ValueError(f'{hv} value heads cannot share {hk} key heads evenly')
+    if not 1 <= dk <= 128:
+        raise ValueError(f'key size {dk} is outside 1 to 128')
+    if not 1 <= dv <= 4096:
+        raise ValueError(f'value size {dv} is outside 1 to 4096')
+    if state is not None:
+        _require_cuda(state, 'state')
+        if state.dtype != torch.float32:
+            raise TypeError(f'the state must be float32, got {state.dtype}')
+        if tuple(state.shape) != (q.shape[0], hv, dk, dv):
+            raise ValueError(f'the state has shape {tuple(state.shape)}, expected {(q.shape[0], hv, dk, dv)}')
+        if state.device != q.device:
+            raise ValueError(f'the state is on {state.device}, q on {q.device}')
+
+
+def delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor, *,
+               scale: Optional[float] = None, initial_state: Optional[torch.Tensor] = None,
+               lengths: Optional[torch.Tensor] = None):
+    """Sequences through plastic synapses.  Returns ``(o, state)``; differentiable (reverse mode, once).
+
+    Parameters
+    ----------
+    q, k : ``(batch, tokens, k_heads, dk)``, float32, bfloat16 or float16, ``dk <= 128``.
+    v : ``(batch, tokens, v_heads, dv)`` of the same type.  ``v_heads`` is a multiple of ``k_heads``;
+        value head ``h`` uses key head ``h // (v_heads // k_heads)``.
+    g, beta : ``(batch, tokens, v_heads)``: logarithm of the decay (``<= 0``) and learning rate.  Cast to float32.
+    scale : factor of the outputs, ``dk ** -0.5`` by default.
+    initial_state : ``(batch, v_heads, dk, dv)`` float32; zero by default.
+    lengths : ``(batch,)`` integers on the device (not read by the host; clipped to ``[0, tokens]``).
+        Tokens of a row from its length on are not read — they may hold anything — and their
+        outputs and gradients are zero.
+
+    ``o`` is ``(batch, tokens, v_heads, dv)`` of the inputs' type, ``state`` the float32 state after each
+    row's last token.  Any strides are taken; a last dimension that is not dense is copied.  Results
+    are the same on every call.
+    """
+    _check(q, k, v, g, beta, initial_state, 2)
+    if lengths is not None:
+        _require_cuda(lengths, 'lengths')
+        if lengths.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f'lengths must be int32 or int64, got {lengths.dtype}')
+        if tuple(lengths.shape) != (q.shape[0],):
+            raise ValueError(f'lengths has shape {tuple(lengths.shape)}, expected {(q.shape[0],)}')
+        if lengths.device != q.device:
+            raise ValueError(f'lengths is on {lengths.device}, q on {q.device}')
+        if lengths.dtype != torch.int32:
+            lengths = lengths.clamp(0, q.shape[1]).to(torch.int32)
+        lengths = lengths.contiguous()
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    g, beta = g.to(torch.float32), beta.to(torch.float32)
+    if initial_state is not None:
+        initial_state = initial_state.contiguous()
+    return _DeltaRule.apply(_dense_rows(q), _dense_rows(k), _dense_rows(v), g, beta, initial_state, lengths,
+                            float(scale))
+
+
+def delta_rule_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
+                    state: torch.Tensor, *, scale: Optional[float] = None) -> torch.Tensor:
+    """One token for every row: ``q, k (batch, k_heads, dk)``, ``v (batch, v_heads, dv)``, ``g, beta (batch,
+    v_heads)``.  ``state`` (dense float32) is updated in place; returns ``o (batch, v_heads, dv)``.
+
+    Not differentiable, since the old state is gone: raises where a gradient would be recorded (use
+    ``delta_rule`` with one token there).
+    """
+    if state is None:
+        raise TypeError('state must be a tensor')
+    _check(q, k, v, g, beta, state, 1)
+    if not state.is_contiguous():
+        raise ValueError('the state must be contiguous: it is updated in place')
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, g, beta, state)):
+        raise RuntimeError('delta_rule_step updates the state in place and records no gradient: '
+                           'use delta_rule, or call it under torch.no_grad()')
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    q, k, v = (_dense_rows(t).unsqueeze(1) for t in (q, k, v))
+    g, beta = g.to(torch.float32).unsqueeze(1), beta.to(torch.float32).unsqueeze(1)
+    o = torch.empty((v.shape[0], *v.shape[2:]), dtype=v.dtype, device=v.device)
+    with torch.cuda.device(v.device):
+        d = _describe(q, k, v, g, beta, state, None, float(scale))
+        check(lib().bsx_delta_recurrent(C.byref(d), ptr(o), ptr(state), _stream(v)))
+    torch.autograd.graph.increment_version(state)
+    return o

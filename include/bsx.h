@@ -547,6 +547,49 @@ int bsx_ipc_free(void* ptr);
 /* The hash behind the background drive, on the host (same integer arithmetic). */
 uint32_t bsx_drive_hash(uint32_t seed, uint32_t neuron, uint32_t step);
 
+/* ---- plastic synapses: the gated delta rule ------------------------------ */
+/* Element types of the dense operators. */
+typedef enum { BSX_T_F32 = 0, BSX_T_BF16 = 1, BSX_T_F16 = 2 } bsx_dtype_t;
+/*
+ * A batch of sequences through a synaptic matrix S (dk, dv) per row and value head that learns
+ * online (error-correcting Hebbian rule with decay; no counterpart in the reference):
+ *   u_t = beta_t (v_t - e^{g_t} S_{t-1}^T k_t),  S_t = e^{g_t} S_{t-1} + k_t u_t^T,  o_t = scale S_t^T q_t
+ * q, k (batch, tokens, k_heads, dk), v (batch, tokens, v_heads, dv) of type dtype; g <= 0 (also
+ * -infinity: the state is dropped) and beta (batch, tokens, v_heads) float32.  Strides of batch,
+ * token and head in elements; the last dimension is dense.  Value head h uses key head
+ * h / (v_heads / k_heads).  initial (batch, v_heads, dk, dv) float32, dense; NULL = zero.
+ * lengths (batch) int32 device values; NULL = tokens.  A row's tokens from its length on are not
+ * read, and its outputs and gradients there are not written.  dk <= 128, dv <= 4096.
+ */
+typedef struct bsx_delta {
+  int64_t batch, tokens;
+  int32_t k_heads, v_heads, dk, dv;
+  int32_t dtype;
+  float scale;
+  const void* q;
+  const void* k;
+  const void* v;
+  const float* g;
+  const float* beta;
+  const float* initial;
+  const int32_t* lengths;
+  int64_t q_stride[3], k_stride[3], v_stride[3], g_stride[3], beta_stride[3];
+} bsx_delta_t;
+/* Chunked form (64 tokens at a time): out (batch, tokens, v_heads, dv) of dtype, dense; state (may
+ * be NULL) receives the state after each row's last token. */
+size_t bsx_delta_workspace_bytes(const bsx_delta_t* desc);
+int bsx_delta_forward(const bsx_delta_t* desc, void* out, float* state, void* workspace, size_t workspace_bytes,
+                      bsx_stream_t stream);
+/* Token by token, for single tokens and short sequences; state may be `initial` itself (in place). */
+int bsx_delta_recurrent(const bsx_delta_t* desc, void* out, float* state, bsx_stream_t stream);
+/* Reverse mode of both: dout as out, dstate (may be NULL) as state; dq, dk, dv of dtype and dg, dbeta
+ * float32, all dense in the shapes of q, k, v, g, beta; dinitial (may be NULL).  Recomputes the
+ * forward pass.  Gradients of shared key heads are summed in head order: results do not vary. */
+size_t bsx_delta_backward_workspace_bytes(const bsx_delta_t* desc);
+int bsx_delta_backward(const bsx_delta_t* desc, const void* dout, const float* dstate, void* dq, void* dk, void* dv,
+                       float* dg, float* dbeta, float* dinitial, void* workspace, size_t workspace_bytes,
+                       bsx_stream_t stream);
+
 /* ---- small utilities ---------------------------------------------------- */
 int bsx_fill_f32(float* dst, int64_t n, float value, bsx_stream_t stream);
 
