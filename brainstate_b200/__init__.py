@@ -11,7 +11,8 @@ from . import event
 from . import nn
 from . import host
 from . import plastic
+from . import quant
 from .event import EventArray, FixedPostNumConn, CSR, FixedPreNumConn, CSC
 
 __version__ = '0.1.0'
-__all__ = ['event', 'nn', 'host', 'plastic', 'EventArray', 'FixedPostNumConn', 'CSR', 'FixedPreNumConn', 'CSC']
+__all__ = ['event', 'nn', 'host', 'plastic', 'quant', 'EventArray', 'FixedPostNumConn', 'CSR', 'FixedPreNumConn', 'CSC']

@@ -24,7 +24,7 @@ BSX_ERR_NONFINITE = -7
 VECMAT_GLOBAL_ATOMICS, VECMAT_SHARED_SLICES = 0, 1
 LINK_EARLY_PUSH, LINK_FETCH_AHEAD, LINK_DEFAULT = 1, 2, 3
 SPK_BOOL8, SPK_F32, SPK_BITS32, SPK_LIST = 0, 1, 2, 3
-T_F32, T_BF16, T_F16 = 0, 1, 2
+T_F32, T_BF16, T_F16, T_EVENT8, T_EVENT32 = 0, 1, 2, 3, 4
 
 
 class BsxError(RuntimeError):
@@ -170,6 +170,13 @@ SIGNATURES = {
     'bsx_delta_recurrent': (_i32, [_deltap, _vp, _vp, _vp]),
     'bsx_delta_backward_workspace_bytes': (_sz, [_deltap]),
     'bsx_delta_backward': (_i32, [_deltap, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    'bsx_int8_row_bytes': (_i64, [_i64]),
+    'bsx_int8_quantize_rows': (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp]),
+    'bsx_int8_quantize_weights': (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _vp]),
+    'bsx_int8_matmul_workspace_bytes': (_sz, [_i64, _i64, _i64]),
+    'bsx_int8_matmul': (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i32, _vp, _sz, _vp]),
+    'bsx_int8_dense_workspace_bytes': (_sz, [_i64, _i64, _i64]),
+    'bsx_int8_dense': (_i32, [_vp, _i32, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _i32, _vp, _sz, _vp]),
     'bsx_fill_f32': (_i32, [_vp, _i64, _f32, _vp]),
 }
 

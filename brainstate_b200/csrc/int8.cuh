@@ -1,0 +1,62 @@
+// Shared parts of the dense 8-bit product (int8_*.cu).
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace bsx {
+namespace int8 {
+
+template <typename E> __device__ __forceinline__ float to_f(E x);
+template <> __device__ __forceinline__ float to_f<float>(float x) { return x; }
+template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <> __device__ __forceinline__ float to_f<__half>(__half x) { return __half2float(x); }
+template <typename E> __device__ __forceinline__ E from_f(float x);
+template <> __device__ __forceinline__ float from_f<float>(float x) { return x; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16(x); }
+template <> __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half(x); }
+
+// The scaled output: the sum is exact, each of the three roundings is 2^-24 of the value.  Factors on both sides of 1
+// are joined first: no intermediate result leaves the range of numbers that the operands and the output lie in.
+template <typename E>
+__device__ __forceinline__ E scaled(int sum, float sx, float sw) {
+  const float s = (float)sum;
+  const bool mixed = (sx < 1.f) != (sw < 1.f);
+  return from_f<E>(__fmul_rn(__fmul_rn(mixed ? sw : s, sx), mixed ? s : sw));
+}
+
+// max|x| of a row or column as the ABI defines its scale: max / 127 in one rounding; NaN where an entry is not finite.
+__device__ __forceinline__ float scale_of(float top, bool finite) {
+  return finite ? __fdiv_rn(top, 127.f) : __int_as_float(0x7fffffff);
+}
+
+// x / s to the nearest integer, ties to even, decided on the exact quotient: the 32-bit product x * (1/s) is within
+// 5e-5 of it, so only values that come within 1e-4 of a border need the 64-bit quotient.
+__device__ __forceinline__ int quantized(float x, float s, float inv) {
+  const float y = x * inv;
+  float n = rintf(y);
+  if (!(fabsf(y - n) < 0.4999f)) n = (float)rint((double)x / (double)s);
+  return (int)fminf(fmaxf(n, -127.f), 127.f);
+}
+
+// Rows of a product's left operand are padded to whole 16-byte stretches.
+inline int64_t padded(int64_t k) { return (k + 15) / 16 * 16; }
+
+struct Product {
+  const int8_t* x;      // (M, Kp)
+  const float* sx;      // (M)
+  const int8_t* w;      // (N, Kp)
+  const float* sw;      // (N)
+  void* out;            // (M, N)
+  int32_t* partial;     // (splits, M, N), or NULL
+  int64_t M, N, Kp;
+};
+
+bool few_applies(int64_t M);
+int launch_few(const Product& p, int dtype, cudaStream_t st);
+int tiles_splits(int64_t M, int64_t N, int64_t Kp, int sms);
+int launch_tiles(const Product& p, int splits, int dtype, cudaStream_t st);
+
+}  // namespace int8
+}  // namespace bsx

@@ -1,0 +1,326 @@
+// Dense 8-bit product: rows of activations and columns of weights to 8 bits, and the C entry points.
+//
+// A row's scale is max|x| / 127 (32 bits); its values are the nearest integers of x / scale.  Spike rows become 0 and 1
+// with scale 1.  A row with an entry that is not finite gets the scale NaN and zeros, so that its outputs are NaN.
+#include "int8.cuh"
+
+namespace bsx {
+namespace int8 {
+
+constexpr int kRowThreads = 256;
+constexpr int kHeld = 4;   // 16-byte stretches a thread keeps between the two passes over its row
+
+template <typename E> struct Stretch { E v[16 / sizeof(E)]; };
+
+// One block per row: the maximum, then the values.  Bound by reading the row once and writing a byte per entry; rows of
+// up to 8192 16-bit or 4096 32-bit entries stay in registers in between, longer ones come from L2 the second time.
+template <typename E, bool VEC>
+__global__ void __launch_bounds__(kRowThreads)
+quantize_rows_kernel(const E* __restrict__ x, int64_t stride, int64_t K, int64_t Kp, int8_t* __restrict__ q,
+                     float* __restrict__ scale) {
+  constexpr int V = 16 / sizeof(E);
+  __shared__ float part[kRowThreads / 32];
+  __shared__ int bad_any;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int64_t row = blockIdx.x;
+  const E* xr = x + row * stride;
+  int8_t* qr = q + row * Kp;
+  if (tid == 0) bad_any = 0;
+  Stretch<E> held[kHeld];
+  float top = 0.f;
+  bool bad = false;
+  if (VEC) {
+    const int64_t n = K / V;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int64_t c = tid + (int64_t)i * kRowThreads;
+      if (c < n) {
+        held[i] = *reinterpret_cast<const Stretch<E>*>(reinterpret_cast<const int4*>(xr) + c);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float a = fabsf(to_f<E>(held[i].v[e]));
+          bad |= !(a <= 3.402823466e38f);
+          top = fmaxf(top, a);
+        }
+      }
+    }
+    for (int64_t c = tid + (int64_t)kHeld * kRowThreads; c < n; c += kRowThreads) {
+      const Stretch<E> h = *reinterpret_cast<const Stretch<E>*>(reinterpret_cast<const int4*>(xr) + c);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float a = fabsf(to_f<E>(h.v[e]));
+        bad |= !(a <= 3.402823466e38f);
+        top = fmaxf(top, a);
+      }
+    }
+  } else {
+    for (int64_t c = tid; c < K; c += kRowThreads) {
+      const float a = fabsf(to_f<E>(xr[c]));
+      bad |= !(a <= 3.402823466e38f);
+      top = fmaxf(top, a);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) part[tid >> 5] = top;
+  __syncthreads();
+  if (bad) bad_any = 1;
+  __syncthreads();
+  top = part[0];
+#pragma unroll
+  for (int w = 1; w < kRowThreads / 32; ++w) top = fmaxf(top, part[w]);
+  const bool finite = bad_any == 0;
+  const float s = scale_of(top, finite);
+  if (tid == 0) scale[row] = s;
+  const bool zero = !finite || s == 0.f;
+  const float inv = s < 1e-30f ? __int_as_float(0x7fffffff) : 1.f / s;   // tiny scales: every quotient in 64 bits
+  if (VEC) {
+    const int64_t n = K / V, np = Kp / V;
+    auto put = [&](int64_t c, const Stretch<E>& h) {
+      uint32_t w[V / 4];
+#pragma unroll
+      for (int e = 0; e < V; e += 4) {
+        uint32_t r = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          r |= (uint32_t)(uint8_t)(int8_t)(zero ? 0 : quantized(to_f<E>(h.v[e + j]), s, inv)) << (8 * j);
+        w[e / 4] = r;
+      }
+      if (V == 8) *reinterpret_cast<uint2*>(qr + c * V) = make_uint2(w[0], w[V / 4 - 1]);
+      else *reinterpret_cast<uint32_t*>(qr + c * V) = w[0];
+    };
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int64_t c = tid + (int64_t)i * kRowThreads;
+      if (c < n) put(c, held[i]);
+    }
+    for (int64_t c = tid + (int64_t)kHeld * kRowThreads; c < n; c += kRowThreads)
+      put(c, *reinterpret_cast<const Stretch<E>*>(reinterpret_cast<const int4*>(xr) + c));
+    for (int64_t c = n + tid; c < np; c += kRowThreads) {
+      if (V == 8) *reinterpret_cast<uint2*>(qr + c * V) = make_uint2(0u, 0u);
+      else *reinterpret_cast<uint32_t*>(qr + c * V) = 0u;
+    }
+  } else {
+    for (int64_t c = tid; c < Kp; c += kRowThreads)
+      qr[c] = (c < K && !zero) ? (int8_t)quantized(to_f<E>(xr[c]), s, inv) : (int8_t)0;
+  }
+}
+
+// Spike rows: 1 where an entry is not zero.
+template <int FORMAT>
+__global__ void __launch_bounds__(kRowThreads)
+event_rows_kernel(const void* __restrict__ x, int64_t stride, int64_t M, int64_t K, int64_t Kp, int8_t* __restrict__ q,
+                  float* __restrict__ scale) {
+  const int64_t words = Kp / 4, total = M * words;
+  for (int64_t i = blockIdx.x * (int64_t)kRowThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kRowThreads) {
+    const int64_t row = i / words, c = (i - row * words) * 4;
+    uint32_t r = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c + j < K && spike_at<FORMAT>(x, row * stride + c + j)) r |= 1u << (8 * j);
+    *reinterpret_cast<uint32_t*>(q + row * Kp + c) = r;
+    if (c == 0) scale[row] = 1.f;
+  }
+}
+
+// Weights (K, N): 32 columns a block, eight rows of threads; the maxima, then 32 x 32 tiles turned through shared memory.
+template <typename E>
+__global__ void __launch_bounds__(256)
+quantize_columns_kernel(const E* __restrict__ w, int64_t K, int64_t N, int64_t Kp, int8_t* __restrict__ q,
+                        float* __restrict__ scale) {
+  __shared__ float top_s[8][32];
+  __shared__ int bad_s[32];
+  __shared__ int8_t tile[32][36];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int64_t n0 = (int64_t)blockIdx.x * 32, n = n0 + tx;
+  if (ty == 0) bad_s[tx] = 0;
+  __syncthreads();
+  float top = 0.f;
+  bool bad = false;
+  if (n < N)
+    for (int64_t k = ty; k < K; k += 8) {
+      const float a = fabsf(to_f<E>(w[k * N + n]));
+      bad |= !(a <= 3.402823466e38f);
+      top = fmaxf(top, a);
+    }
+  top_s[ty][tx] = top;
+  if (bad) bad_s[tx] = 1;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, top_s[i][tx]);
+  const bool finite = bad_s[tx] == 0;
+  const float s = scale_of(top, finite);
+  if (ty == 0 && n < N) scale[n] = s;
+  const bool zero = !finite || s == 0.f;
+  const float inv = s < 1e-30f ? __int_as_float(0x7fffffff) : 1.f / s;
+  for (int64_t k0 = 0; k0 < Kp; k0 += 32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t k = k0 + ty + 8 * i;
+      tile[tx][ty + 8 * i] = (n < N && k < K && !zero) ? (int8_t)quantized(to_f<E>(w[k * N + n]), s, inv) : (int8_t)0;
+    }
+    __syncthreads();
+    const int r = threadIdx.x >> 3, c = (threadIdx.x & 7) * 4;
+    if (n0 + r < N && k0 + c < Kp)
+      *reinterpret_cast<uint32_t*>(q + (n0 + r) * Kp + k0 + c) = *reinterpret_cast<const uint32_t*>(&tile[r][c]);
+    __syncthreads();
+  }
+}
+
+template <typename E>
+static int launch_rows(const void* x, int64_t stride, int64_t M, int64_t K, int8_t* q, float* scale, cudaStream_t st) {
+  const int64_t Kp = padded(K);
+  constexpr int V = 16 / sizeof(E);
+  const E* p = static_cast<const E*>(x);
+  if (aligned16(x) && (M == 1 || stride % V == 0) && K % V == 0)
+    quantize_rows_kernel<E, true><<<(unsigned)M, kRowThreads, 0, st>>>(p, stride, K, Kp, q, scale);
+  else
+    quantize_rows_kernel<E, false><<<(unsigned)M, kRowThreads, 0, st>>>(p, stride, K, Kp, q, scale);
+  BSX_LAUNCH_CHECK("quantize_rows_kernel");
+  return BSX_OK;
+}
+
+static int rows(const void* x, int format, int64_t stride, int64_t M, int64_t K, int8_t* q, float* scale, cudaStream_t st) {
+  switch (format) {
+    case BSX_T_F32: return launch_rows<float>(x, stride, M, K, q, scale, st);
+    case BSX_T_BF16: return launch_rows<__nv_bfloat16>(x, stride, M, K, q, scale, st);
+    case BSX_T_F16: return launch_rows<__half>(x, stride, M, K, q, scale, st);
+    default: break;
+  }
+  const int64_t Kp = padded(K), want = (M * (Kp / 4) + kRowThreads - 1) / kRowThreads, most = 16ll * sm_count();
+  const unsigned grid = (unsigned)(want < most ? want : most);
+  if (format == BSX_T_EVENT8)
+    event_rows_kernel<BSX_SPK_BOOL8><<<grid, kRowThreads, 0, st>>>(x, stride, M, K, Kp, q, scale);
+  else
+    event_rows_kernel<BSX_SPK_F32><<<grid, kRowThreads, 0, st>>>(x, stride, M, K, Kp, q, scale);
+  BSX_LAUNCH_CHECK("event_rows_kernel");
+  return BSX_OK;
+}
+
+static int check_sizes(int64_t M, int64_t K, int64_t N) {
+  if (M < 0 || K < 0 || N < 0) return fail(BSX_ERR_INVALID_ARG, "negative size");
+  if (M > INT32_MAX || N > INT32_MAX) return fail(BSX_ERR_UNSUPPORTED, "sizes must fit int32");
+  // |sum| <= 127^2 K has to fit 32 bits
+  if (K > 131072) return fail(BSX_ERR_UNSUPPORTED, "more than 131072 inputs: sums would leave 32 bits");
+  return BSX_OK;
+}
+static int check_format(int format) {
+  if (format < BSX_T_F32 || format > BSX_T_EVENT32) return fail(BSX_ERR_INVALID_ARG, "unknown element type");
+  return BSX_OK;
+}
+
+static size_t aligned(size_t n) { return (n + 255) / 256 * 256; }
+
+// Bytes of the parts of the workspace: rows in 8 bits, their scales, partial sums.
+static size_t partial_bytes(int64_t M, int64_t K, int64_t N, int sms) {
+  if (few_applies(M)) return 0;
+  const int splits = tiles_splits(M, N, padded(K), sms);
+  return splits > 1 ? (size_t)splits * M * N * sizeof(int32_t) : 0;
+}
+
+static int product(const int8_t* q, const float* sx, const int8_t* w, const float* sw, int64_t M, int64_t K, int64_t N,
+                   void* out, int out_type, void* partial, cudaStream_t st) {
+  Product p;
+  p.x = q; p.sx = sx; p.w = w; p.sw = sw; p.out = out;
+  p.partial = static_cast<int32_t*>(partial);
+  p.M = M; p.N = N; p.Kp = padded(K);
+  if (few_applies(M)) return launch_few(p, out_type, st);
+  return launch_tiles(p, tiles_splits(M, N, p.Kp, sm_count()), out_type, st);
+}
+
+}  // namespace int8
+}  // namespace bsx
+
+using namespace bsx;
+using namespace bsx::int8;
+
+extern "C" int64_t bsx_int8_row_bytes(int64_t K) { return K < 0 ? 0 : padded(K); }
+
+extern "C" int bsx_int8_quantize_rows(const void* x, int format, int64_t row_stride, int64_t M, int64_t K, int8_t* q,
+                                      float* scale, bsx_stream_t stream) {
+  BSX_TRACE("bsx_int8_quantize_rows");
+  int rc;
+  if ((rc = check_sizes(M, K, 0)) != BSX_OK || (rc = check_format(format)) != BSX_OK) return rc;
+  if (M == 0) return BSX_OK;
+  if ((K > 0 && (!x || !q)) || !scale) return fail(BSX_ERR_INVALID_ARG, "NULL buffer");
+  if (K > 0 && !aligned16(q)) return fail(BSX_ERR_INVALID_ARG, "q must start on a 16-byte boundary");
+  if (sm_count() <= 0) return fail(BSX_ERR_CUDA, "no CUDA device");
+  if (K == 0) return fail(BSX_ERR_UNSUPPORTED, "rows without entries have no scale");
+  return rows(x, format, row_stride, M, K, q, scale, as_stream(stream));
+}
+
+extern "C" int bsx_int8_quantize_weights(const void* w, int dtype, int64_t K, int64_t N, int8_t* q, float* scale,
+                                         bsx_stream_t stream) {
+  BSX_TRACE("bsx_int8_quantize_weights");
+  int rc;
+  if ((rc = check_sizes(0, K, N)) != BSX_OK) return rc;
+  if (dtype < BSX_T_F32 || dtype > BSX_T_F16) return fail(BSX_ERR_INVALID_ARG, "unknown element type");
+  if (N == 0) return BSX_OK;
+  if (K == 0) return fail(BSX_ERR_UNSUPPORTED, "columns without entries have no scale");
+  if (!w || !q || !scale) return fail(BSX_ERR_INVALID_ARG, "NULL buffer");
+  if (!aligned16(q)) return fail(BSX_ERR_INVALID_ARG, "q must start on a 16-byte boundary");
+  if (sm_count() <= 0) return fail(BSX_ERR_CUDA, "no CUDA device");
+  cudaStream_t st = as_stream(stream);
+  const unsigned grid = (unsigned)((N + 31) / 32);
+  const int64_t Kp = padded(K);
+  if (dtype == BSX_T_F32)
+    quantize_columns_kernel<float><<<grid, 256, 0, st>>>(static_cast<const float*>(w), K, N, Kp, q, scale);
+  else if (dtype == BSX_T_BF16)
+    quantize_columns_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(w), K, N, Kp, q, scale);
+  else
+    quantize_columns_kernel<__half><<<grid, 256, 0, st>>>(static_cast<const __half*>(w), K, N, Kp, q, scale);
+  BSX_LAUNCH_CHECK("quantize_columns_kernel");
+  return BSX_OK;
+}
+
+extern "C" size_t bsx_int8_matmul_workspace_bytes(int64_t M, int64_t K, int64_t N) {
+  return check_sizes(M, K, N) == BSX_OK ? partial_bytes(M, K, N, sm_count()) : 0;
+}
+
+extern "C" int bsx_int8_matmul(const int8_t* q, const float* scale, const int8_t* wq, const float* wscale, int64_t M,
+                               int64_t K, int64_t N, void* out, int out_dtype, void* ws, size_t ws_bytes,
+                               bsx_stream_t stream) {
+  BSX_TRACE("bsx_int8_matmul");
+  int rc;
+  if ((rc = check_sizes(M, K, N)) != BSX_OK) return rc;
+  if (out_dtype < BSX_T_F32 || out_dtype > BSX_T_F16) return fail(BSX_ERR_INVALID_ARG, "unknown output type");
+  if (M == 0 || N == 0) return BSX_OK;
+  if (K == 0) return fail(BSX_ERR_UNSUPPORTED, "product over no inputs");
+  if (!q || !scale || !wq || !wscale || !out) return fail(BSX_ERR_INVALID_ARG, "NULL buffer");
+  if (!aligned16(q) || !aligned16(wq)) return fail(BSX_ERR_INVALID_ARG, "8-bit operands must start on a 16-byte boundary");
+  const int sms = sm_count();
+  if (sms <= 0) return fail(BSX_ERR_CUDA, "no CUDA device");
+  const size_t need = partial_bytes(M, K, N, sms);
+  if (need > 0 && (!ws || !aligned16(ws) || ws_bytes < need))
+    return fail(BSX_ERR_WORKSPACE, "workspace missing, misaligned or too small");
+  return product(q, scale, wq, wscale, M, K, N, out, out_dtype, ws, as_stream(stream));
+}
+
+extern "C" size_t bsx_int8_dense_workspace_bytes(int64_t M, int64_t K, int64_t N) {
+  if (check_sizes(M, K, N) != BSX_OK) return 0;
+  return aligned((size_t)M * padded(K)) + aligned((size_t)M * sizeof(float)) + partial_bytes(M, K, N, sm_count());
+}
+
+extern "C" int bsx_int8_dense(const void* x, int format, int64_t row_stride, const int8_t* wq, const float* wscale,
+                              int64_t M, int64_t K, int64_t N, void* out, int out_dtype, void* ws, size_t ws_bytes,
+                              bsx_stream_t stream) {
+  BSX_TRACE("bsx_int8_dense");
+  int rc;
+  if ((rc = check_sizes(M, K, N)) != BSX_OK || (rc = check_format(format)) != BSX_OK) return rc;
+  if (out_dtype < BSX_T_F32 || out_dtype > BSX_T_F16) return fail(BSX_ERR_INVALID_ARG, "unknown output type");
+  if (M == 0 || N == 0) return BSX_OK;
+  if (K == 0) return fail(BSX_ERR_UNSUPPORTED, "product over no inputs");
+  if (!x || !wq || !wscale || !out) return fail(BSX_ERR_INVALID_ARG, "NULL buffer");
+  if (!aligned16(wq)) return fail(BSX_ERR_INVALID_ARG, "8-bit operands must start on a 16-byte boundary");
+  const int sms = sm_count();
+  if (sms <= 0) return fail(BSX_ERR_CUDA, "no CUDA device");
+  const size_t qb = aligned((size_t)M * padded(K)), sb = aligned((size_t)M * sizeof(float));
+  if (!ws || !aligned16(ws) || ws_bytes < qb + sb + partial_bytes(M, K, N, sms))
+    return fail(BSX_ERR_WORKSPACE, "workspace missing, misaligned or too small");
+  char* base = static_cast<char*>(ws);
+  int8_t* q = reinterpret_cast<int8_t*>(base);
+  float* sx = reinterpret_cast<float*>(base + qb);
+  cudaStream_t st = as_stream(stream);
+  if ((rc = rows(x, format, row_stride, M, K, q, sx, st)) != BSX_OK) return rc;
+  return product(q, sx, wq, wscale, M, K, N, out, out_dtype, base + qb + sb, st);
+}

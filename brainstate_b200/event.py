@@ -67,7 +67,7 @@ class EventArray:
         if isinstance(other, torch.Tensor):       # dense event product (EventLinear)
             from .nn._event_linear import dense_event_matmul
             return dense_event_matmul(self.value, other)
-        return NotImplemented
+        return NotImplemented                     # containers of other modules take it from the right
 
 
 class _Transposed:

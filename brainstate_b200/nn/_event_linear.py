@@ -17,12 +17,13 @@ import numpy as np
 import torch
 
 from .. import _lib
-from ..event import _flatten_batch, _require_cuda, spike_format_of
+from ..event import EventArray, _flatten_batch, _require_cuda, spike_format_of
+from ..quant import Int8Dense, int8_matmul
 from ._event_fixedprob import _device, _init_weight
 from ._module import Module, Size
 from ._state import ParamState
 
-__all__ = ['EventLinear', 'dense_event_matmul']
+__all__ = ['EventLinear', 'Int8Linear', 'dense_event_matmul']
 
 
 class _DenseEvent(torch.autograd.Function):
@@ -155,3 +156,38 @@ class EventLinear(Module):
         if self.float_as_event:
             return dense_event_matmul(spk, weight)
         return spk.to(torch.float32) @ weight
+
+    def quantized(self) -> 'Int8Linear':
+        """The serving form of the layer: a copy of its present weights in 8 bits."""
+        weight = self.weight.value
+        if weight.numel() == 1:
+            raise ValueError('a layer of one weight is not quantised')
+        return Int8Linear(self.in_size, self.out_size, weight, float_as_event=self.float_as_event, name=self.name)
+
+
+class Int8Linear(Module):
+    """Dense layer in 8-bit integers: ``EventLinear`` for serving (see :mod:`brainstate_b200.quant`).  ``weight``:
+    ``(n_pre, n_post)`` floats or an ``Int8Dense``.  With ``float_as_event`` every entry of the input that is not zero is a
+    spike; otherwise float rows are quantised on the way (bool and uint8 inputs are spikes either way).  Not
+    differentiable."""
+
+    __module__ = 'brainstate_b200.nn'
+
+    def __init__(self, in_size: Size, out_size: Size, weight: Union[np.ndarray, torch.Tensor, Int8Dense],
+                 float_as_event: bool = False, name: Optional[str] = None, device=None):
+        super().__init__(name=name)
+        self.in_size = in_size
+        self.out_size = out_size
+        self.float_as_event = float_as_event
+        if not isinstance(weight, Int8Dense):
+            if not isinstance(weight, torch.Tensor):
+                weight = torch.as_tensor(np.asarray(weight, dtype=np.float32), device=_device(device))
+            weight = Int8Dense(weight)
+        if weight.shape != (self.in_size[-1], self.out_size[-1]):
+            raise ValueError(f'weight has shape {weight.shape}, expected {(self.in_size[-1], self.out_size[-1])}')
+        self.weight = weight
+
+    def update(self, x: torch.Tensor) -> torch.Tensor:
+        if self.float_as_event or x.dtype in (torch.bool, torch.uint8):
+            return int8_matmul(EventArray(x), self.weight)
+        return int8_matmul(x, self.weight)

@@ -548,8 +548,9 @@ int bsx_ipc_free(void* ptr);
 uint32_t bsx_drive_hash(uint32_t seed, uint32_t neuron, uint32_t step);
 
 /* ---- plastic synapses: the gated delta rule ------------------------------ */
-/* Element types of the dense operators. */
-typedef enum { BSX_T_F32 = 0, BSX_T_BF16 = 1, BSX_T_F16 = 2 } bsx_dtype_t;
+/* Element types of the dense operators; the last two mark spike rows (a byte or a float32 per
+ * neuron, not zero = spike). */
+typedef enum { BSX_T_F32 = 0, BSX_T_BF16 = 1, BSX_T_F16 = 2, BSX_T_EVENT8 = 3, BSX_T_EVENT32 = 4 } bsx_dtype_t;
 /*
  * A batch of sequences through a synaptic matrix S (dk, dv) per row and value head that learns
  * online (error-correcting Hebbian rule with decay; no counterpart in the reference):
@@ -589,6 +590,33 @@ size_t bsx_delta_backward_workspace_bytes(const bsx_delta_t* desc);
 int bsx_delta_backward(const bsx_delta_t* desc, const void* dout, const float* dstate, void* dq, void* dk, void* dv,
                        float* dg, float* dbeta, float* dinitial, void* workspace, size_t workspace_bytes,
                        bsx_stream_t stream);
+
+/* ---- dense product in 8-bit integers ------------------------------------- */
+/*
+ * The serving form of a trained dense layer x @ W (brainstate/nn/_event_linear.py:97-102), W (K, N):
+ * weights with a scale per output channel, activations with a scale per row, integer sums.
+ *   scale = max|.| / 127 (float32), q = nearest integer of value / scale (ties to even; decided on the
+ *   exact quotient), out = (sum_k q_x q_w) * scale_x * scale_w
+ * Spike rows (BSX_T_EVENT8, BSX_T_EVENT32) are 0 and 1 with scale 1.  A row or channel with an entry that
+ * is not finite gets the scale NaN; one of zeros the scale 0.  Rows of 8-bit values are padded with
+ * zeros to bsx_int8_row_bytes(K) bytes and start on 16-byte boundaries.  1 <= K <= 131072.
+ */
+int64_t bsx_int8_row_bytes(int64_t K);
+/* x (M, K), rows row_stride elements apart -> q (M, bsx_int8_row_bytes(K)), scale (M). */
+int bsx_int8_quantize_rows(const void* x, int format, int64_t row_stride, int64_t M, int64_t K, int8_t* q, float* scale,
+                           bsx_stream_t stream);
+/* W (K, N) dense, F32, BF16 or F16 -> q (N, bsx_int8_row_bytes(K)), scale (N). */
+int bsx_int8_quantize_weights(const void* w, int dtype, int64_t K, int64_t N, int8_t* q, float* scale, bsx_stream_t stream);
+/* Rows already in 8 bits; out (M, N) dense, F32, BF16 or F16.  The workspace (may be 0 bytes) holds
+ * partial sums where a long inner dimension is split. */
+size_t bsx_int8_matmul_workspace_bytes(int64_t M, int64_t K, int64_t N);
+int bsx_int8_matmul(const int8_t* q, const float* scale, const int8_t* wq, const float* wscale, int64_t M, int64_t K,
+                    int64_t N, void* out, int out_dtype, void* workspace, size_t workspace_bytes, bsx_stream_t stream);
+/* Both: x (M, K) of the given format. */
+size_t bsx_int8_dense_workspace_bytes(int64_t M, int64_t K, int64_t N);
+int bsx_int8_dense(const void* x, int format, int64_t row_stride, const int8_t* wq, const float* wscale, int64_t M,
+                   int64_t K, int64_t N, void* out, int out_dtype, void* workspace, size_t workspace_bytes,
+                   bsx_stream_t stream);
 
 /* ---- small utilities ---------------------------------------------------- */
 int bsx_fill_f32(float* dst, int64_t n, float value, bsx_stream_t stream);
