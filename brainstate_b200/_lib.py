@@ -102,7 +102,6 @@ _i64, _i32, _vp, _sz, _f32 = C.c_int64, C.c_int, C.c_void_p, C.c_size_t, C.c_flo
 _connp = C.POINTER(BsxConn)
 _netp = C.POINTER(BsxNet)
 _lifp = C.POINTER(BsxLifParams)
-_deltap = C.POINTER(BsxDelta)
 
 # name -> (restype, argtypes); every symbol include/bsx.h declares, plus the two tuning hooks of
 # csrc/bsx_tuning.h (INTERNAL lists them)
@@ -165,11 +164,12 @@ SIGNATURES = {
     'bsx_ipc_close': (_i32, [_vp]),
     'bsx_ipc_free': (_i32, [_vp]),
     'bsx_drive_hash': (C.c_uint32, [C.c_uint32, C.c_uint32, C.c_uint32]),
-    'bsx_delta_workspace_bytes': (_sz, [_deltap]),
-    'bsx_delta_forward': (_i32, [_deltap, _vp, _vp, _vp, _sz, _vp]),
-    'bsx_delta_recurrent': (_i32, [_deltap, _vp, _vp, _vp]),
-    'bsx_delta_backward_workspace_bytes': (_sz, [_deltap]),
-    'bsx_delta_backward': (_i32, [_deltap, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    # the description of a delta rule call may be a BsxDelta or its bytes
+    'bsx_delta_workspace_bytes': (_sz, [_vp]),
+    'bsx_delta_forward': (_i32, [_vp, _vp, _vp, _vp, _sz, _vp]),
+    'bsx_delta_recurrent': (_i32, [_vp, _vp, _vp, _vp]),
+    'bsx_delta_backward_workspace_bytes': (_sz, [_vp]),
+    'bsx_delta_backward': (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     'bsx_int8_row_bytes': (_i64, [_i64]),
     'bsx_int8_quantize_rows': (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp]),
     'bsx_int8_quantize_weights': (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _vp]),
@@ -217,3 +217,15 @@ def current_stream() -> int:
 def ptr(t) -> int | None:
     """Device address of a torch tensor (``None`` passes NULL)."""
     return None if t is None else t.data_ptr()
+
+
+def call_on(device: int, fn, *args) -> None:
+    """``fn(*args, stream)`` of the library on a device's current stream, checked.  Makes the device current for the call
+    where it is not."""
+    import torch
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    if torch._C._cuda_getDevice() == device:
+        check(fn(*args, stream))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, stream))

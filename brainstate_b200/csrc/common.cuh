@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "bsx.h"
 
 #if defined(__CUDA_ARCH__) && (__CUDA_ARCH__ < 1000)
@@ -46,6 +48,19 @@ int cuda_fail(cudaError_t e, const char* what);
 int check_conn(const bsx_conn_t* c);
 // Number of SMs of the current device (148 on B200); <= 0 on failure.
 int sm_count();
+
+// Lets a kernel use up to `bytes` of dynamic shared memory on the current device; `seen` (a static of the caller, one
+// per kernel) remembers the devices where it was done for the most bytes the caller ever asks for.
+template <typename F>
+inline int allow_smem(F kernel, size_t bytes, std::atomic<uint64_t>& seen) {
+  int dev = 0;
+  BSX_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (seen.load(std::memory_order_relaxed) & bit) return BSX_OK;
+  BSX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  seen.fetch_or(bit, std::memory_order_relaxed);
+  return BSX_OK;
+}
 
 inline cudaStream_t as_stream(bsx_stream_t s) { return reinterpret_cast<cudaStream_t>(s); }
 

@@ -51,12 +51,36 @@ struct Product {
   void* out;            // (M, N)
   int32_t* partial;     // (splits, M, N), or NULL
   int64_t M, N, Kp;
+  bool after_rows;      // launched right behind the kernel that writes x and sx: may start before that has ended
 };
 
-bool few_applies(int64_t M);
+// A product's kernel is launched while the kernel that quantises its rows still runs, sets itself up (and asks for
+// weights, which that kernel does not touch), and waits here for the rows.
+__device__ __forceinline__ void let_dependents_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_rows() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... P, typename... A>
+inline cudaError_t launch_behind(bool early, void (*kernel)(P...), unsigned grid, unsigned threads, size_t smem,
+                                 cudaStream_t st, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = early ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
+struct Plan { int rows, splits; };
+
+bool few_applies(int64_t M, int64_t N, int64_t Kp);
 int launch_few(const Product& p, int dtype, cudaStream_t st);
-int tiles_splits(int64_t M, int64_t N, int64_t Kp, int sms);
-int launch_tiles(const Product& p, int splits, int dtype, cudaStream_t st);
+Plan plan_tiles(int64_t M, int64_t N, int64_t Kp, int sms);
+int launch_tiles(const Product& p, Plan plan, int dtype, cudaStream_t st);
 
 }  // namespace int8
 }  // namespace bsx

@@ -7,118 +7,139 @@
 namespace bsx {
 namespace int8 {
 
-constexpr int kRowThreads = 256;
-constexpr int kHeld = 4;   // 16-byte stretches a thread keeps between the two passes over its row
+constexpr int kHeld = 2;   // 16-byte stretches a thread keeps between the two passes over its row
 
 template <typename E> struct Stretch { E v[16 / sizeof(E)]; };
 
-// One block per row: the maximum, then the values.  Bound by reading the row once and writing a byte per entry; rows of
-// up to 8192 16-bit or 4096 32-bit entries stay in registers in between, longer ones come from L2 the second time.
-template <typename E, bool VEC>
-__global__ void __launch_bounds__(kRowThreads)
+__device__ __forceinline__ bool note(float x, float& top) {   // true for what is not finite
+  const float a = fabsf(x);
+  top = fmaxf(top, a);
+  return !(a <= 3.402823466e38f);
+}
+
+// Four values in one word.  The nearest integer comes from the sum with 1.5 * 2^23, whose low byte is it; where a value
+// comes near a border the exact rule decides, out of line.
+__device__ __noinline__ uint32_t four_exact(float4 x, float s, float inv) {
+  return (uint32_t)(uint8_t)(int8_t)quantized(x.x, s, inv) | (uint32_t)(uint8_t)(int8_t)quantized(x.y, s, inv) << 8 |
+         (uint32_t)(uint8_t)(int8_t)quantized(x.z, s, inv) << 16 | (uint32_t)(uint8_t)(int8_t)quantized(x.w, s, inv) << 24;
+}
+__device__ __forceinline__ uint32_t four(float4 x, float s, float inv) {
+  constexpr float M = 12582912.f;
+  const float y0 = x.x * inv, y1 = x.y * inv, y2 = x.z * inv, y3 = x.w * inv;
+  const float t0 = __fadd_rn(y0, M), t1 = __fadd_rn(y1, M), t2 = __fadd_rn(y2, M), t3 = __fadd_rn(y3, M);
+  const float d = fmaxf(fmaxf(fabsf(y0 - __fsub_rn(t0, M)), fabsf(y1 - __fsub_rn(t1, M))),
+                        fmaxf(fabsf(y2 - __fsub_rn(t2, M)), fabsf(y3 - __fsub_rn(t3, M))));
+  if (!(d < 0.4999f)) return four_exact(x, s, inv);
+  return __byte_perm(__byte_perm(__float_as_uint(t0), __float_as_uint(t1), 0x0040),
+                     __byte_perm(__float_as_uint(t2), __float_as_uint(t3), 0x0040), 0x5410);
+}
+
+// One block per row: the maximum, then the values.  Bound by reading the row once and writing a byte per entry; the first
+// kHeld 16-byte stretches of a thread stay in registers in between, the rest comes from L2 the second time.
+template <typename E, bool VEC, int THREADS>
+__global__ void __launch_bounds__(THREADS)
 quantize_rows_kernel(const E* __restrict__ x, int64_t stride, int64_t K, int64_t Kp, int8_t* __restrict__ q,
                      float* __restrict__ scale) {
   constexpr int V = 16 / sizeof(E);
-  __shared__ float part[kRowThreads / 32];
-  __shared__ int bad_any;
+  __shared__ float part[THREADS / 32];
   const int tid = threadIdx.x, lane = tid & 31;
   const int64_t row = blockIdx.x;
   const E* xr = x + row * stride;
   int8_t* qr = q + row * Kp;
-  if (tid == 0) bad_any = 0;
+  let_dependents_start();
   Stretch<E> held[kHeld];
   float top = 0.f;
   bool bad = false;
+  const int n = (int)(K / V);
+  const int4* x4 = reinterpret_cast<const int4*>(xr);
   if (VEC) {
-    const int64_t n = K / V;
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-      const int64_t c = tid + (int64_t)i * kRowThreads;
-      if (c < n) {
-        held[i] = *reinterpret_cast<const Stretch<E>*>(reinterpret_cast<const int4*>(xr) + c);
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float a = fabsf(to_f<E>(held[i].v[e]));
-          bad |= !(a <= 3.402823466e38f);
-          top = fmaxf(top, a);
-        }
+    for (int i = 0; i < kHeld; ++i)
+      if (tid + i * THREADS < n) {
+        const int4 w = __ldg(x4 + tid + i * THREADS);
+        held[i] = *reinterpret_cast<const Stretch<E>*>(&w);
       }
-    }
-    for (int64_t c = tid + (int64_t)kHeld * kRowThreads; c < n; c += kRowThreads) {
-      const Stretch<E> h = *reinterpret_cast<const Stretch<E>*>(reinterpret_cast<const int4*>(xr) + c);
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float a = fabsf(to_f<E>(h.v[e]));
-        bad |= !(a <= 3.402823466e38f);
-        top = fmaxf(top, a);
+    for (int i = 0; i < kHeld; ++i)
+      if (tid + i * THREADS < n) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) bad |= note(to_f<E>(held[i].v[e]), top);
       }
+    for (int c = tid + kHeld * THREADS; c < n; c += THREADS) {
+      const int4 w = __ldg(x4 + c);
+      const Stretch<E> h = *reinterpret_cast<const Stretch<E>*>(&w);
+#pragma unroll
+      for (int e = 0; e < V; ++e) bad |= note(to_f<E>(h.v[e]), top);
     }
   } else {
-    for (int64_t c = tid; c < K; c += kRowThreads) {
-      const float a = fabsf(to_f<E>(xr[c]));
-      bad |= !(a <= 3.402823466e38f);
-      top = fmaxf(top, a);
-    }
+    for (int c = tid; c < K; c += THREADS) bad |= note(to_f<E>(xr[c]), top);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (lane == 0) part[tid >> 5] = top;
-  __syncthreads();
-  if (bad) bad_any = 1;
-  __syncthreads();
-  top = part[0];
+  const bool finite = !__syncthreads_or(bad);
+  top = part[lane % (THREADS / 32)];
 #pragma unroll
-  for (int w = 1; w < kRowThreads / 32; ++w) top = fmaxf(top, part[w]);
-  const bool finite = bad_any == 0;
+  for (int o = THREADS / 64; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   const float s = scale_of(top, finite);
   if (tid == 0) scale[row] = s;
   const bool zero = !finite || s == 0.f;
   const float inv = s < 1e-30f ? __int_as_float(0x7fffffff) : 1.f / s;   // tiny scales: every quotient in 64 bits
   if (VEC) {
-    const int64_t n = K / V, np = Kp / V;
-    auto put = [&](int64_t c, const Stretch<E>& h) {
+    auto put = [&](int c, const Stretch<E>& h) {
       uint32_t w[V / 4];
 #pragma unroll
-      for (int e = 0; e < V; e += 4) {
-        uint32_t r = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          r |= (uint32_t)(uint8_t)(int8_t)(zero ? 0 : quantized(to_f<E>(h.v[e + j]), s, inv)) << (8 * j);
-        w[e / 4] = r;
-      }
-      if (V == 8) *reinterpret_cast<uint2*>(qr + c * V) = make_uint2(w[0], w[V / 4 - 1]);
-      else *reinterpret_cast<uint32_t*>(qr + c * V) = w[0];
+      for (int e = 0; e < V; e += 4)
+        w[e / 4] = zero ? 0u : four(make_float4(to_f<E>(h.v[e]), to_f<E>(h.v[e + 1]), to_f<E>(h.v[e + 2]), to_f<E>(h.v[e + 3])),
+                                    s, inv);
+      if (V == 8) reinterpret_cast<uint2*>(qr)[c] = make_uint2(w[0], w[V / 4 - 1]);
+      else reinterpret_cast<uint32_t*>(qr)[c] = w[0];
     };
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-      const int64_t c = tid + (int64_t)i * kRowThreads;
-      if (c < n) put(c, held[i]);
+    for (int i = 0; i < kHeld; ++i)
+      if (tid + i * THREADS < n) put(tid + i * THREADS, held[i]);
+    for (int c = tid + kHeld * THREADS; c < n; c += THREADS) {
+      const int4 w = __ldg(x4 + c);
+      put(c, *reinterpret_cast<const Stretch<E>*>(&w));
     }
-    for (int64_t c = tid + (int64_t)kHeld * kRowThreads; c < n; c += kRowThreads)
-      put(c, *reinterpret_cast<const Stretch<E>*>(reinterpret_cast<const int4*>(xr) + c));
-    for (int64_t c = n + tid; c < np; c += kRowThreads) {
-      if (V == 8) *reinterpret_cast<uint2*>(qr + c * V) = make_uint2(0u, 0u);
-      else *reinterpret_cast<uint32_t*>(qr + c * V) = 0u;
+    for (int c = n + tid; c < (int)(Kp / V); c += THREADS) {
+      if (V == 8) reinterpret_cast<uint2*>(qr)[c] = make_uint2(0u, 0u);
+      else reinterpret_cast<uint32_t*>(qr)[c] = 0u;
     }
   } else {
-    for (int64_t c = tid; c < Kp; c += kRowThreads)
-      qr[c] = (c < K && !zero) ? (int8_t)quantized(to_f<E>(xr[c]), s, inv) : (int8_t)0;
+    for (int c = tid * 4; c < Kp; c += THREADS * 4) {
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = c + j < K ? to_f<E>(xr[c + j]) : 0.f;
+      *reinterpret_cast<uint32_t*>(qr + c) = zero ? 0u : four(make_float4(v[0], v[1], v[2], v[3]), s, inv);
+    }
   }
 }
 
-// Spike rows: 1 where an entry is not zero.
-template <int FORMAT>
-__global__ void __launch_bounds__(kRowThreads)
+// Spike rows: 1 where an entry is not zero; 16 entries a thread.
+template <int FORMAT, bool VEC>
+__global__ void __launch_bounds__(256)
 event_rows_kernel(const void* __restrict__ x, int64_t stride, int64_t M, int64_t K, int64_t Kp, int8_t* __restrict__ q,
                   float* __restrict__ scale) {
-  const int64_t words = Kp / 4, total = M * words;
-  for (int64_t i = blockIdx.x * (int64_t)kRowThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kRowThreads) {
-    const int64_t row = i / words, c = (i - row * words) * 4;
-    uint32_t r = 0;
+  let_dependents_start();
+  const int64_t words = Kp / 16, total = M * words;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / words, c = (i - row * words) * 16;
+    uint4 r;
+    if (VEC && FORMAT == BSX_SPK_BOOL8) {
+      r = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(x) + row * stride + c));
+      r.x = __vsetgtu4(r.x, 0u);
+      r.y = __vsetgtu4(r.y, 0u);
+      r.z = __vsetgtu4(r.z, 0u);
+      r.w = __vsetgtu4(r.w, 0u);
+    } else {
+      uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (c + j < K && spike_at<FORMAT>(x, row * stride + c + j)) r |= 1u << (8 * j);
-    *reinterpret_cast<uint32_t*>(q + row * Kp + c) = r;
+      for (int j = 0; j < 16; ++j)
+        if (c + j < K && spike_at<FORMAT>(x, row * stride + c + j)) w[j / 4] |= 1u << (8 * (j % 4));
+      r = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    *reinterpret_cast<uint4*>(q + row * Kp + c) = r;
     if (c == 0) scale[row] = 1.f;
   }
 }
@@ -167,15 +188,22 @@ quantize_columns_kernel(const E* __restrict__ w, int64_t K, int64_t N, int64_t K
   }
 }
 
+template <typename E, bool VEC>
+static void launch_rows_vec(const E* x, int64_t stride, int64_t M, int64_t K, int8_t* q, float* scale, cudaStream_t st) {
+  const int64_t Kp = padded(K);
+  // few rows: the time is that of one row, so that as many threads as its stretches fill share it
+  if (M < 148 && K * (int64_t)sizeof(E) > 256 * 16)
+    quantize_rows_kernel<E, VEC, 1024><<<(unsigned)M, 1024, 0, st>>>(x, stride, K, Kp, q, scale);
+  else
+    quantize_rows_kernel<E, VEC, 256><<<(unsigned)M, 256, 0, st>>>(x, stride, K, Kp, q, scale);
+}
+
 template <typename E>
 static int launch_rows(const void* x, int64_t stride, int64_t M, int64_t K, int8_t* q, float* scale, cudaStream_t st) {
-  const int64_t Kp = padded(K);
   constexpr int V = 16 / sizeof(E);
   const E* p = static_cast<const E*>(x);
-  if (aligned16(x) && (M == 1 || stride % V == 0) && K % V == 0)
-    quantize_rows_kernel<E, true><<<(unsigned)M, kRowThreads, 0, st>>>(p, stride, K, Kp, q, scale);
-  else
-    quantize_rows_kernel<E, false><<<(unsigned)M, kRowThreads, 0, st>>>(p, stride, K, Kp, q, scale);
+  if (aligned16(x) && (M == 1 || stride % V == 0) && K % V == 0) launch_rows_vec<E, true>(p, stride, M, K, q, scale, st);
+  else launch_rows_vec<E, false>(p, stride, M, K, q, scale, st);
   BSX_LAUNCH_CHECK("quantize_rows_kernel");
   return BSX_OK;
 }
@@ -187,12 +215,14 @@ static int rows(const void* x, int format, int64_t stride, int64_t M, int64_t K,
     case BSX_T_F16: return launch_rows<__half>(x, stride, M, K, q, scale, st);
     default: break;
   }
-  const int64_t Kp = padded(K), want = (M * (Kp / 4) + kRowThreads - 1) / kRowThreads, most = 16ll * sm_count();
+  const int64_t Kp = padded(K), want = (M * (Kp / 16) + 255) / 256, most = 8ll * sm_count();
   const unsigned grid = (unsigned)(want < most ? want : most);
-  if (format == BSX_T_EVENT8)
-    event_rows_kernel<BSX_SPK_BOOL8><<<grid, kRowThreads, 0, st>>>(x, stride, M, K, Kp, q, scale);
+  if (format == BSX_T_EVENT32)
+    event_rows_kernel<BSX_SPK_F32, false><<<grid, 256, 0, st>>>(x, stride, M, K, Kp, q, scale);
+  else if (aligned16(x) && (M == 1 || stride % 16 == 0) && K % 16 == 0)
+    event_rows_kernel<BSX_SPK_BOOL8, true><<<grid, 256, 0, st>>>(x, stride, M, K, Kp, q, scale);
   else
-    event_rows_kernel<BSX_SPK_F32><<<grid, kRowThreads, 0, st>>>(x, stride, M, K, Kp, q, scale);
+    event_rows_kernel<BSX_SPK_BOOL8, false><<<grid, 256, 0, st>>>(x, stride, M, K, Kp, q, scale);
   BSX_LAUNCH_CHECK("event_rows_kernel");
   return BSX_OK;
 }
@@ -213,19 +243,20 @@ static size_t aligned(size_t n) { return (n + 255) / 256 * 256; }
 
 // Bytes of the parts of the workspace: rows in 8 bits, their scales, partial sums.
 static size_t partial_bytes(int64_t M, int64_t K, int64_t N, int sms) {
-  if (few_applies(M)) return 0;
-  const int splits = tiles_splits(M, N, padded(K), sms);
+  if (few_applies(M, N, padded(K))) return 0;
+  const int splits = plan_tiles(M, N, padded(K), sms).splits;
   return splits > 1 ? (size_t)splits * M * N * sizeof(int32_t) : 0;
 }
 
-static int product(const int8_t* q, const float* sx, const int8_t* w, const float* sw, int64_t M, int64_t K, int64_t N,
+static int product(bool after_rows, const int8_t* q, const float* sx, const int8_t* w, const float* sw, int64_t M, int64_t K, int64_t N,
                    void* out, int out_type, void* partial, cudaStream_t st) {
   Product p;
   p.x = q; p.sx = sx; p.w = w; p.sw = sw; p.out = out;
   p.partial = static_cast<int32_t*>(partial);
   p.M = M; p.N = N; p.Kp = padded(K);
-  if (few_applies(M)) return launch_few(p, out_type, st);
-  return launch_tiles(p, tiles_splits(M, N, p.Kp, sm_count()), out_type, st);
+  p.after_rows = after_rows;
+  if (few_applies(M, N, p.Kp)) return launch_few(p, out_type, st);
+  return launch_tiles(p, plan_tiles(M, N, p.Kp, sm_count()), out_type, st);
 }
 
 }  // namespace int8
@@ -293,7 +324,7 @@ extern "C" int bsx_int8_matmul(const int8_t* q, const float* scale, const int8_t
   const size_t need = partial_bytes(M, K, N, sms);
   if (need > 0 && (!ws || !aligned16(ws) || ws_bytes < need))
     return fail(BSX_ERR_WORKSPACE, "workspace missing, misaligned or too small");
-  return product(q, scale, wq, wscale, M, K, N, out, out_dtype, ws, as_stream(stream));
+  return product(false, q, scale, wq, wscale, M, K, N, out, out_dtype, ws, as_stream(stream));
 }
 
 extern "C" size_t bsx_int8_dense_workspace_bytes(int64_t M, int64_t K, int64_t N) {
@@ -322,5 +353,5 @@ extern "C" int bsx_int8_dense(const void* x, int format, int64_t row_stride, con
   float* sx = reinterpret_cast<float*>(base + qb);
   cudaStream_t st = as_stream(stream);
   if ((rc = rows(x, format, row_stride, M, K, q, sx, st)) != BSX_OK) return rc;
-  return product(q, sx, wq, wscale, M, K, N, out, out_dtype, base + qb + sb, st);
+  return product(true, q, sx, wq, wscale, M, K, N, out, out_dtype, base + qb + sb, st);
 }

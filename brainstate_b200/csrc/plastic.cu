@@ -47,6 +47,15 @@ static int fill(const bsx_delta_t* d, Args& a) {
     a.qs[i] = d->q_stride[i]; a.ks[i] = d->k_stride[i]; a.vs[i] = d->v_stride[i];
     a.gs[i] = d->g_stride[i]; a.bs[i] = d->beta_stride[i];
   }
+  // the stride of a dimension of one entry says nothing and must not spoil the alignment rule
+  auto single = [](int64_t* s, int64_t batch, int64_t tokens, int64_t heads) {
+    if (batch == 1) s[0] = 0;
+    if (tokens == 1) s[1] = 0;
+    if (heads == 1) s[2] = 0;
+  };
+  single(a.qs, d->batch, d->tokens, d->k_heads);
+  single(a.ks, d->batch, d->tokens, d->k_heads);
+  single(a.vs, d->batch, d->tokens, d->v_heads);
   a.T = d->tokens; a.B = (int)d->batch; a.Hk = d->k_heads; a.Hv = d->v_heads; a.dk = d->dk; a.dv = d->dv;
   a.NC = (int)chunks_of(d->tokens);
   a.scale = d->scale;

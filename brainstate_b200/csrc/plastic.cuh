@@ -183,12 +183,5 @@ int launch_scan(const Args& a, int dtype, bool save, cudaStream_t st);
 int launch_backward_scan(const Args& a, int dtype, cudaStream_t st);
 int launch_backward_chunks(const Args& a, int dtype, cudaStream_t st);
 
-// Lets a kernel use `bytes` of dynamic shared memory.
-template <typename F>
-inline int allow_smem(F kernel, size_t bytes) {
-  BSX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-  return BSX_OK;
-}
-
 }  // namespace plastic
 }  // namespace bsx

@@ -293,7 +293,8 @@ __global__ void __launch_bounds__(256) backward_scan_kernel(Args a, int groups) 
 template <typename E, int DK, int WS>
 static int launch_scan_one(const Args& a, int groups, cudaStream_t st) {
   const size_t bytes = BackScanLayout<E, DK>::bytes(groups, WS);
-  int rc = allow_smem(backward_scan_kernel<E, DK, WS>, bytes);
+  static std::atomic<uint64_t> seen;
+  int rc = allow_smem(backward_scan_kernel<E, DK, WS>, kMaxSmem, seen);
   if (rc != BSX_OK) return rc;
   const int per_head = (a.dv + 16 * groups - 1) / (16 * groups);
   const unsigned grid = (unsigned)((int64_t)a.B * a.Hv * per_head);
@@ -750,7 +751,8 @@ __global__ void __launch_bounds__(256) head_sum_kernel(Args a) {
 template <typename E, int DK>
 static int launch_chunks_typed(const Args& a, cudaStream_t st) {
   const size_t bytes = BackChunkLayout<E, DK>::bytes;
-  int rc = allow_smem(backward_chunk_kernel<E, DK>, bytes);
+  static std::atomic<uint64_t> seen;
+  int rc = allow_smem(backward_chunk_kernel<E, DK>, bytes, seen);
   if (rc != BSX_OK) return rc;
   backward_chunk_kernel<E, DK><<<(unsigned)((int64_t)a.B * a.Hv * a.NC), 256, bytes, st>>>(a);
   BSX_LAUNCH_CHECK("plastic backward_chunk_kernel");

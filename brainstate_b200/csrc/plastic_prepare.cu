@@ -185,12 +185,13 @@ template <typename E, int DK>
 static int launch_typed(const Args& a, bool backward, cudaStream_t st) {
   const size_t bytes = PrepLayout<E, DK>::bytes;
   const unsigned grid = (unsigned)((int64_t)a.B * a.Hv * a.NC);
+  static std::atomic<uint64_t> seen[2];
   int rc;
   if (backward) {
-    if ((rc = allow_smem(prepare_kernel<E, DK, true>, bytes)) != BSX_OK) return rc;
+    if ((rc = allow_smem(prepare_kernel<E, DK, true>, bytes, seen[1])) != BSX_OK) return rc;
     prepare_kernel<E, DK, true><<<grid, 128, bytes, st>>>(a);
   } else {
-    if ((rc = allow_smem(prepare_kernel<E, DK, false>, bytes)) != BSX_OK) return rc;
+    if ((rc = allow_smem(prepare_kernel<E, DK, false>, bytes, seen[0])) != BSX_OK) return rc;
     prepare_kernel<E, DK, false><<<grid, 128, bytes, st>>>(a);
   }
   BSX_LAUNCH_CHECK("plastic prepare_kernel");

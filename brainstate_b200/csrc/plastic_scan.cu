@@ -314,7 +314,8 @@ __global__ void __launch_bounds__(256) scan_kernel(Args a, int groups) {
 template <typename E, int DK, int WS, bool OUT, bool SAVE>
 static int launch_one(const Args& a, int groups, cudaStream_t st) {
   const size_t bytes = ScanLayout<E, DK, OUT>::bytes(groups, WS);
-  int rc = allow_smem(scan_kernel<E, DK, WS, OUT, SAVE>, bytes);
+  static std::atomic<uint64_t> seen;
+  int rc = allow_smem(scan_kernel<E, DK, WS, OUT, SAVE>, kMaxSmem, seen);
   if (rc != BSX_OK) return rc;
   const int per_head = (a.dv + 16 * groups - 1) / (16 * groups);
   const unsigned grid = (unsigned)((int64_t)a.B * a.Hv * per_head);

@@ -17,19 +17,20 @@ have a norm of at most about 1 and ``beta`` lie in [0, 1] (the rule diverges whe
 """
 from __future__ import annotations
 
-import ctypes as C
+import struct
 from typing import Optional
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import BsxDelta, check, lib, ptr
+from ._lib import call_on, lib
 from .event import _require_cuda
 
 __all__ = ['delta_rule', 'delta_rule_step']
 
 _TYPES = {torch.float32: _lib.T_F32, torch.bfloat16: _lib.T_BF16, torch.float16: _lib.T_F16}
+_DESC = struct.Struct('=2q5if7Q15q')       # bsx_delta_t
 
 # Sequences of at most this many tokens go token by token (one launch, the state read and written
 # once) instead of by chunks.
@@ -37,55 +38,42 @@ RECURRENT_TOKENS = 16
 
 
 def _dense_rows(t: torch.Tensor) -> torch.Tensor:
-    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
-def _strides(t: torch.Tensor):
-    # the stride of a dimension of one entry says nothing and must not spoil the alignment rule
-    return tuple(0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3]))
+def _describe(q, k, v, g, beta, initial, lengths, scale) -> bytes:
+    B, T, Hk, dk = q.shape
+    Hv, dv = v.shape[2:]
+    return _DESC.pack(B, T, Hk, Hv, dk, dv, _TYPES[q.dtype], scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
+                      beta.data_ptr(), 0 if initial is None else initial.data_ptr(),
+                      0 if lengths is None else lengths.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+                      *g.stride(), *beta.stride())
 
 
-def _describe(q, k, v, g, beta, initial, lengths, scale) -> BsxDelta:
-    d = BsxDelta()
-    d.batch, d.tokens, d.k_heads, d.dk = q.shape
-    d.v_heads, d.dv = v.shape[2:]
-    d.dtype, d.scale = _TYPES[q.dtype], scale
-    d.q, d.k, d.v, d.g, d.beta = q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr()
-    d.initial, d.lengths = ptr(initial), ptr(lengths)
-    d.q_stride[:], d.k_stride[:], d.v_stride[:] = _strides(q), _strides(k), _strides(v)
-    d.g_stride[:], d.beta_stride[:] = _strides(g), _strides(beta)
-    return d
-
-
-def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+def _forward(q, k, v, g, beta, initial, lengths, scale):
+    B, T, _, dk = q.shape
+    Hv, dv = v.shape[2:]
+    # tokens past a row's length are not written by the kernels
+    o = v.new_empty((B, T, Hv, dv)) if lengths is None else v.new_zeros((B, T, Hv, dv))
+    state = g.new_empty((B, Hv, dk, dv))
+    d = _describe(q, k, v, g, beta, initial, lengths, scale)
+    if T <= RECURRENT_TOKENS:
+        call_on(v.get_device(), lib().bsx_delta_recurrent, d, o.data_ptr(), state.data_ptr())
+    else:
+        n = lib().bsx_delta_workspace_bytes(d)
+        ws = g.new_empty(n // 4)
+        call_on(v.get_device(), lib().bsx_delta_forward, d, o.data_ptr(), state.data_ptr(), ws.data_ptr(), n)
+    return o, state
 
 
 class _DeltaRule(torch.autograd.Function):
 
     @staticmethod
-    def forward(q, k, v, g, beta, initial, lengths, scale):
-        B, T, _, dk = q.shape
-        Hv, dv = v.shape[2:]
-        # tokens past a row's length are not written by the kernels
-        o = (torch.empty if lengths is None else torch.zeros)((B, T, Hv, dv), dtype=v.dtype, device=v.device)
-        state = torch.empty((B, Hv, dk, dv), dtype=torch.float32, device=v.device)
-        with torch.cuda.device(v.device):
-            d = _describe(q, k, v, g, beta, initial, lengths, scale)
-            if T <= RECURRENT_TOKENS:
-                check(lib().bsx_delta_recurrent(C.byref(d), ptr(o), ptr(state), _stream(v)))
-            else:
-                n = lib().bsx_delta_workspace_bytes(C.byref(d))
-                ws = torch.empty(n, dtype=torch.uint8, device=v.device)
-                check(lib().bsx_delta_forward(C.byref(d), ptr(o), ptr(state), ptr(ws), n, _stream(v)))
-        return o, state
-
-    @staticmethod
-    def setup_context(ctx, inputs, output):
-        q, k, v, g, beta, initial, lengths, scale = inputs
+    def forward(ctx, q, k, v, g, beta, initial, lengths, scale):
         ctx.scale = scale
         ctx.save_for_backward(q, k, v, g, beta, initial, lengths)
         ctx.set_materialize_grads(False)
+        return _forward(q, k, v, g, beta, initial, lengths, scale)
 
     @staticmethod
     @once_differentiable
@@ -93,25 +81,44 @@ class _DeltaRule(torch.autograd.Function):
         if do is None and dstate is None:
             return (None,) * 8
         q, k, v, g, beta, initial, lengths = ctx.saved_tensors
-        make = torch.empty if lengths is None else torch.zeros
-        if do is None:
-            do = torch.zeros((*v.shape,), dtype=v.dtype, device=v.device)
-        do = do.contiguous()
+        ragged = lengths is not None
+        # dense whatever the strides of the inputs; tokens past a row's length are not written by the kernels
+        dq, dk, dv, dg, dbeta = (t.new_zeros(t.shape) if ragged else t.new_empty(t.shape) for t in (q, k, v, g, beta))
+        do = v.new_zeros(v.shape) if do is None else do.contiguous()
         dstate = None if dstate is None else dstate.contiguous()
-        dq, dk, dv = (make(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        dg, dbeta = (make(t.shape, dtype=torch.float32, device=t.device) for t in (g, beta))
-        dinitial = torch.empty_like(initial) if ctx.needs_input_grad[5] else None
-        with torch.cuda.device(v.device):
-            d = _describe(q, k, v, g, beta, initial, lengths, ctx.scale)
-            n = lib().bsx_delta_backward_workspace_bytes(C.byref(d))
-            ws = torch.empty(max(n, 1), dtype=torch.uint8, device=v.device)
-            check(lib().bsx_delta_backward(C.byref(d), ptr(do), ptr(dstate), ptr(dq), ptr(dk), ptr(dv), ptr(dg),
-                                           ptr(dbeta), ptr(dinitial), ptr(ws), n, _stream(v)))
+        dinitial = initial.new_empty(initial.shape) if ctx.needs_input_grad[5] else None
+        d = _describe(q, k, v, g, beta, initial, lengths, ctx.scale)
+        n = lib().bsx_delta_backward_workspace_bytes(d)
+        ws = g.new_empty(n // 4)
+        call_on(v.get_device(), lib().bsx_delta_backward, d, do.data_ptr(), None if dstate is None else dstate.data_ptr(),
+                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(), dbeta.data_ptr(),
+                None if dinitial is None else dinitial.data_ptr(), ws.data_ptr(), n)
         return dq, dk, dv, dg, dbeta, dinitial, None, None
 
 
+def _fits(q, k, v, g, beta, state, lead: int) -> bool:
+    """Whether the kernels take the arguments; ``lead`` is the number of dimensions before the heads."""
+    try:
+        qs, vs, gs, dev = q.shape, v.shape, g.shape, q.get_device()
+        return (dev >= 0 and k.get_device() == dev and v.get_device() == dev and g.get_device() == dev
+                and beta.get_device() == dev and q.dtype in _TYPES and k.dtype == q.dtype and v.dtype == q.dtype
+                and g.dtype.is_floating_point and beta.dtype.is_floating_point and len(qs) == lead + 2
+                and k.shape == qs and len(vs) == lead + 2 and vs[:lead] == qs[:lead] and gs == vs[:-1] and beta.shape == gs
+                and qs[lead] > 0 and vs[lead] > 0 and vs[lead] % qs[lead] == 0 and 1 <= qs[-1] <= 128
+                and 1 <= vs[-1] <= 4096
+                and (state is None or (state.dtype == torch.float32 and state.get_device() == dev
+                                       and tuple(state.shape) == (qs[0], vs[lead], qs[-1], vs[-1]))))
+    except AttributeError:
+        return False
+
+
 def _check(q, k, v, g, beta, state, lead: int):
-    """Refuses what the kernels do not take; ``lead`` is the number of dimensions before the heads."""
+    if not _fits(q, k, v, g, beta, state, lead):
+        _refuse(q, k, v, g, beta, state, lead)
+
+
+def _refuse(q, k, v, g, beta, state, lead: int):
+    """Says what does not fit."""
     for name, t, dims in (('q', q, lead + 2), ('k', k, lead + 2), ('v', v, lead + 2), ('g', g, lead + 1),
                           ('beta', beta, lead + 1)):
         if not isinstance(t, torch.Tensor):
@@ -143,6 +150,8 @@ def _check(q, k, v, g, beta, state, lead: int):
     if not 1 <= dv <= 4096:
         raise ValueError(f'value size {dv} is outside 1 to 4096')
     if state is not None:
+        if not isinstance(state, torch.Tensor):
+            raise TypeError('state must be a tensor')
         _require_cuda(state, 'state')
         if state.dtype != torch.float32:
             raise TypeError(f'the state must be float32, got {state.dtype}')
@@ -185,13 +194,17 @@ def delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
         if lengths.dtype != torch.int32:
             lengths = lengths.clamp(0, q.shape[1]).to(torch.int32)
         lengths = lengths.contiguous()
-    if scale is None:
-        scale = q.shape[-1] ** -0.5
-    g, beta = g.to(torch.float32), beta.to(torch.float32)
+    if g.dtype != torch.float32:
+        g = g.to(torch.float32)
+    if beta.dtype != torch.float32:
+        beta = beta.to(torch.float32)
     if initial_state is not None:
         initial_state = initial_state.contiguous()
-    return _DeltaRule.apply(_dense_rows(q), _dense_rows(k), _dense_rows(v), g, beta, initial_state, lengths,
-                            float(scale))
+    args = (_dense_rows(q), _dense_rows(k), _dense_rows(v), g, beta, initial_state, lengths,
+            q.shape[-1] ** -0.5 if scale is None else float(scale))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:6]):
+        return _DeltaRule.apply(*args)
+    return _forward(*args)
 
 
 def delta_rule_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
@@ -210,13 +223,17 @@ def delta_rule_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, g, beta, state)):
         raise RuntimeError('delta_rule_step updates the state in place and records no gradient: '
                            'use delta_rule, or call it under torch.no_grad()')
-    if scale is None:
-        scale = q.shape[-1] ** -0.5
-    q, k, v = (_dense_rows(t).unsqueeze(1) for t in (q, k, v))
-    g, beta = g.to(torch.float32).unsqueeze(1), beta.to(torch.float32).unsqueeze(1)
-    o = torch.empty((v.shape[0], *v.shape[2:]), dtype=v.dtype, device=v.device)
-    with torch.cuda.device(v.device):
-        d = _describe(q, k, v, g, beta, state, None, float(scale))
-        check(lib().bsx_delta_recurrent(C.byref(d), ptr(o), ptr(state), _stream(v)))
+    q, k, v = _dense_rows(q), _dense_rows(k), _dense_rows(v)
+    if g.dtype != torch.float32:
+        g = g.to(torch.float32)
+    if beta.dtype != torch.float32:
+        beta = beta.to(torch.float32)
+    (B, Hk, dk), (_, Hv, dv) = q.shape, v.shape
+    o = v.new_empty((B, Hv, dv))
+    (qb, qh, _), (kb, kh, _), (vb, vh, _), (gb, gh), (bb, bh) = q.stride(), k.stride(), v.stride(), g.stride(), beta.stride()
+    at = state.data_ptr()
+    d = _DESC.pack(B, 1, Hk, Hv, dk, dv, _TYPES[q.dtype], dk ** -0.5 if scale is None else scale, q.data_ptr(), k.data_ptr(),
+                   v.data_ptr(), g.data_ptr(), beta.data_ptr(), at, 0, qb, 0, qh, kb, 0, kh, vb, 0, vh, gb, 0, gh, bb, 0, bh)
+    call_on(v.get_device(), lib().bsx_delta_recurrent, d, o.data_ptr(), at)
     torch.autograd.graph.increment_version(state)
     return o

@@ -15,17 +15,13 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._lib import check, lib, ptr
+from ._lib import call_on, lib
 from .event import EventArray, _require_cuda
 
 __all__ = ['Int8Dense', 'Int8Rows', 'quantize_rows', 'int8_matmul']
 
 _TYPES = {torch.float32: _lib.T_F32, torch.bfloat16: _lib.T_BF16, torch.float16: _lib.T_F16}
 _EVENTS = {torch.bool: _lib.T_EVENT8, torch.uint8: _lib.T_EVENT8, torch.float32: _lib.T_EVENT32}
-
-
-def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
 
 
 def _rows(x, n: Optional[int]):
@@ -80,8 +76,8 @@ def quantize_rows(x) -> Int8Rows:
     m, n = x2.shape
     q = torch.empty((m, lib().bsx_int8_row_bytes(n)), dtype=torch.int8, device=x2.device)
     scale = torch.empty(m, dtype=torch.float32, device=x2.device)
-    with torch.cuda.device(x2.device):
-        check(lib().bsx_int8_quantize_rows(ptr(x2), fmt, x2.stride(0), m, n, ptr(q), ptr(scale), _stream(x2)))
+    call_on(x2.get_device(), lib().bsx_int8_quantize_rows, x2.data_ptr(), fmt, x2.stride(0), m, n, q.data_ptr(),
+            scale.data_ptr())
     return Int8Rows(q, scale, n, lead, torch.float32 if isinstance(x, EventArray) else x2.dtype)
 
 
@@ -102,11 +98,10 @@ class Int8Dense:
             raise ValueError('a matrix without inputs cannot be quantised')
         w = weight.detach().contiguous()
         self.shape = (int(w.shape[0]), int(w.shape[1]))
-        with torch.cuda.device(w.device):
-            self.q = torch.empty((self.shape[1], lib().bsx_int8_row_bytes(self.shape[0])), dtype=torch.int8, device=w.device)
-            self.scale = torch.empty(self.shape[1], dtype=torch.float32, device=w.device)
-            check(lib().bsx_int8_quantize_weights(ptr(w), _TYPES[w.dtype], *self.shape, ptr(self.q), ptr(self.scale),
-                                                  _stream(w)))
+        self.q = torch.empty((self.shape[1], lib().bsx_int8_row_bytes(self.shape[0])), dtype=torch.int8, device=w.device)
+        self.scale = torch.empty(self.shape[1], dtype=torch.float32, device=w.device)
+        call_on(w.get_device(), lib().bsx_int8_quantize_weights, w.data_ptr(), _TYPES[w.dtype], *self.shape,
+                self.q.data_ptr(), self.scale.data_ptr())
 
     def dequantize(self) -> torch.Tensor:
         """The float32 weights that the integers stand for."""
@@ -115,6 +110,14 @@ class Int8Dense:
     def __rmatmul__(self, x):
         if isinstance(x, (torch.Tensor, EventArray)):
             return int8_matmul(x, self)
+        return NotImplemented
+
+    @classmethod
+    def __torch_function__(cls, func, types, args=(), kwargs=None):
+        # ``tensor @ w`` comes here first; sent on, it would reach __rmatmul__ only after an error was raised and dropped
+        if func in (torch.Tensor.__matmul__, torch.Tensor.matmul, torch.matmul) and not kwargs and len(args) == 2 \
+                and isinstance(args[1], cls):
+            return int8_matmul(*args)
         return NotImplemented
 
 
@@ -136,19 +139,18 @@ def int8_matmul(x, w: Int8Dense, out_dtype: Optional[torch.dtype] = None) -> tor
     kind = kind if out_dtype is None else out_dtype
     if kind not in _TYPES:
         raise TypeError(f'out_dtype must be float32, bfloat16 or float16, got {kind}')
-    if data.device != w.q.device:
+    if data.get_device() != w.q.get_device():
         raise ValueError(f'input is on {data.device}, the weights on {w.q.device}')
-    m = data.shape[0]
-    out = torch.empty((m, n_post), dtype=kind, device=data.device)
-    with torch.cuda.device(data.device):
-        if rows:
-            n = lib().bsx_int8_matmul_workspace_bytes(m, n_pre, n_post)
-            ws = torch.empty(n, dtype=torch.uint8, device=data.device) if n else None
-            check(lib().bsx_int8_matmul(ptr(data), ptr(x.scale), ptr(w.q), ptr(w.scale), m, n_pre, n_post, ptr(out),
-                                        _TYPES[kind], ptr(ws), n, _stream(data)))
-        else:
-            n = lib().bsx_int8_dense_workspace_bytes(m, n_pre, n_post)
-            ws = torch.empty(n, dtype=torch.uint8, device=data.device)
-            check(lib().bsx_int8_dense(ptr(data), fmt, data.stride(0), ptr(w.q), ptr(w.scale), m, n_pre, n_post, ptr(out),
-                                       _TYPES[kind], ptr(ws), n, _stream(data)))
-    return out.reshape(lead + (n_post,))
+    m, dev = data.shape[0], data.get_device()
+    out = data.new_empty(lead + (n_post,), dtype=kind)
+    if rows:
+        n = lib().bsx_int8_matmul_workspace_bytes(m, n_pre, n_post)
+        ws = data.new_empty(n) if n else None
+        call_on(dev, lib().bsx_int8_matmul, data.data_ptr(), x.scale.data_ptr(), w.q.data_ptr(), w.scale.data_ptr(), m, n_pre,
+                n_post, out.data_ptr(), _TYPES[kind], None if ws is None else ws.data_ptr(), n)
+    else:
+        n = lib().bsx_int8_dense_workspace_bytes(m, n_pre, n_post)
+        ws = w.q.new_empty(n)
+        call_on(dev, lib().bsx_int8_dense, data.data_ptr(), fmt, data.stride(0), w.q.data_ptr(), w.scale.data_ptr(), m, n_pre,
+                n_post, out.data_ptr(), _TYPES[kind], ws.data_ptr(), n)
+    return out
