@@ -11,9 +11,10 @@ static int width_of(int dk) { return dk <= 64 ? 64 : 128; }
 
 static size_t workspace(const bsx_delta_t* d, bool backward) {
   const int64_t n = d->batch * d->v_heads * chunks_of(d->tokens);
-  size_t f = (size_t)n * (2 * kC * kC + kVec);
+  const size_t size = d->dtype == BSX_T_F32 ? 4 : 2;
+  size_t f = (size_t)n * kRecord + (size_t)(n / (d->v_heads / d->k_heads)) * (2 * kC * (width_of(d->dk) + 8) * size / 4);
   if (backward) {
-    f += (size_t)n * (kC * kC + 2 * (size_t)d->dv * (width_of(d->dk) + kC));
+    f += (size_t)n * (kTri + 2 * (size_t)d->dv * (width_of(d->dk) + kC));
     if (d->k_heads != d->v_heads) f += 2 * (size_t)d->batch * d->tokens * d->v_heads * d->dk;
   }
   return f * sizeof(float);
@@ -64,18 +65,16 @@ static int fill(const bsx_delta_t* d, Args& a) {
     return aligned16(p) && s[0] % per == 0 && s[1] % per == 0 && s[2] % per == 0 && cols % per == 0;
   };
   a.vec_qk = vec(a.q, a.qs, a.dk) && vec(a.k, a.ks, a.dk);
-  a.vec_v = vec(a.v, a.vs, a.dv);
   return BSX_OK;
 }
 
 static void place(Args& a, const bsx_delta_t* d, float* ws, bool backward) {
   const int64_t n = (int64_t)a.B * a.Hv * a.NC;
-  a.Tm = ws; ws += n * kC * kC;
-  a.Pm = ws; ws += n * kC * kC;
-  a.vec = ws; ws += n * kVec;
+  a.kq = ws; ws += (int64_t)a.B * a.Hk * a.NC * (2 * kC * (width_of(a.dk) + 8) * (d->dtype == BSX_T_F32 ? 4 : 2) / 4);
+  a.rec = ws; ws += n * kRecord;
   if (!backward) return;
   const int64_t wide = width_of(a.dk);
-  a.Bm = ws; ws += n * kC * kC;
+  a.Bm = ws; ws += n * kTri;
   a.Sn = ws; ws += n * a.dv * wide;
   a.dS = ws; ws += n * a.dv * wide;
   a.U = ws; ws += n * a.dv * kC;
@@ -148,8 +147,6 @@ extern "C" int bsx_delta_backward(const bsx_delta_t* d, const void* dout, const 
   if (sm_count() <= 0) return fail(BSX_ERR_CUDA, "no CUDA device");
   a.dout = dout; a.dstate = dstate;
   a.dq = dq; a.dk_ = dk; a.dv_ = dv; a.dg = dg; a.dbeta = dbeta; a.dinitial = dinitial;
-  const int per = d->dtype == BSX_T_F32 ? 4 : 8;
-  a.vec_do = aligned16(dout) && a.dv % per == 0;
   place(a, d, static_cast<float*>(ws), true);
   cudaStream_t st = as_stream(stream);
   if (a.NC > 0) {

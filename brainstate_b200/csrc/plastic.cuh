@@ -17,14 +17,17 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "bulk_copy.cuh"
 #include "common.cuh"
 
 namespace bsx {
 namespace plastic {
 
 constexpr int kC = 64;           // tokens of a chunk
-constexpr size_t kMaxSmem = 227 * 1024;   // dynamic shared memory of a block
+constexpr size_t kMaxSmem = 227 * 1024 - 64;   // dynamic shared memory of a block, beside its few static bytes
 constexpr int kVec = 5 * kC;     // e^G, e^{G_C-G}, beta, G (high part), G (low part)
+constexpr int kTri = 36 * 64;    // lower triangle of a 64x64 matrix: 8x8 tiles by rows, each row-major
+constexpr int kRecord = 2 * kTri + kVec;   // T, P and the vectors of a chunk, one contiguous record
 
 struct Args {
   const void *q, *k, *v;
@@ -34,8 +37,10 @@ struct Args {
   int64_t T;
   int B, Hk, Hv, dk, dv, NC;
   float scale;
-  // per (row, head, chunk): T, P, A / beta (64 x 64 each; entries above the diagonal blocks are not written), vectors
-  float *Tm, *Pm, *Bm, *vec;
+  // per (row, key head, chunk): K and Q tiles, 64 rows of DK + 8 elements each, as they lie in shared memory
+  void* kq;
+  // per (row, value head, chunk): T, P and vectors (kRecord floats); A / beta (kTri), backward only
+  float *rec, *Bm;
   // per (row, head, chunk), transposed: state before the chunk (dv, DK), U (dv, 64); backward only
   float *Sn, *U;
   void* o;
@@ -47,7 +52,7 @@ struct Args {
   void *dq, *dk_, *dv_;
   float *dg, *dbeta, *dinitial;
   float *dq32, *dk32;     // per value head, when heads share keys
-  bool vec_qk, vec_v, vec_do;
+  bool vec_qk;            // rows of q and k start on 16-byte boundaries and are whole 16-byte stretches
 };
 
 template <typename E> __device__ __forceinline__ float to_f(E x);
@@ -145,6 +150,7 @@ template <int N> __device__ __forceinline__ void cp_wait() {
 
 // Stages `rows` (of 64) token rows x `cols` (of COLS) of a (token, column) tile; the rest is zero.  vec: rows start on
 // 16-byte boundaries and cols is a multiple of a 16-byte stretch.
+// (used where the tiles are first read, by the kernel that packs them)
 template <typename E>
 __device__ __forceinline__ void stage(E* sm, int pitch, const E* src, int64_t stride, int rows, int cols, int colspad,
                                       bool vec, int tid, int nthr) {
@@ -163,19 +169,101 @@ __device__ __forceinline__ void stage(E* sm, int pitch, const E* src, int64_t st
     }
   }
 }
-// Stages the lower block triangle (16x16 blocks) of a 64x64 matrix.
-__device__ __forceinline__ void stage_lower(float* sm, int pitch, const float* src, int tid, int nthr) {
-  for (int i = tid; i < kC * 16; i += nthr) {
-    const int r = i >> 4, c = (i & 15) * 4;
-    if (c < ((r >> 4) + 1) * 16) cp16(sm + r * pitch + c, src + r * kC + c, true);
+// Place of 8x8 tile (row tile n, column tile k <= n) in a packed lower triangle.
+__device__ __forceinline__ constexpr int tri(int n, int k) { return (n * (n + 1) / 2 + k) * 64; }
+
+// Waits for the bytes of a stage; false when the bounded wait ran out (the caller then spoils its results with NaN).
+__device__ __forceinline__ bool stage_wait(uint64_t* bar, uint32_t parity) {
+  for (uint32_t i = 0; i < (1u << 20); ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return false;
+}
+
+// Operand tiles (16 value columns x 8) handed from one warp of a group to the others, already split: 1 KB a tile, in
+// the order of a left operand's registers.
+__device__ __forceinline__ void put_split(float4* base, int tile, int lane, const float* c) {
+  float h[4], l[4];
+  split4(c, h, l);
+  base[tile * 64 + lane] = make_float4(h[0], l[0], h[2], l[2]);
+  base[tile * 64 + 32 + lane] = make_float4(h[1], l[1], h[3], l[3]);
+}
+__device__ __forceinline__ void get_split(const float4* base, int tile, int lane, float* hi, float* lo) {
+  const float4 x = base[tile * 64 + lane], y = base[tile * 64 + 32 + lane];
+  hi[0] = x.x; lo[0] = x.y; hi[1] = x.z; lo[1] = x.w;
+  hi[2] = y.x; lo[2] = y.y; hi[3] = y.z; lo[3] = y.w;
+}
+
+// Right-operand tiles from a (row, column) tile in shared memory: N 8x8 tiles whose rows are the outer index (pairs of
+// neighbouring columns) ...
+__device__ __forceinline__ float2 unpack(uint32_t w, const __nv_bfloat16*) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ float2 unpack(uint32_t w, const __half*) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+// ... and N tiles side by side whose rows are the inner index (pairs of neighbouring rows).
+template <int N, typename E>
+__device__ __forceinline__ void tiles_by_row(float2* b, const E* at, int pitch, int lane) {
+  if constexpr (sizeof(E) == 2) {
+    uint32_t r[4];
+    const uint32_t addr = smem_u32(at + (lane & 7) * pitch + ((lane >> 3) % N) * 8);
+    if constexpr (N == 4)
+      asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+    else
+      asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
+#pragma unroll
+    for (int n = 0; n < N; ++n) b[n] = unpack(r[n], at);
+  } else {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int n = 0; n < N; ++n) b[n] = make_float2(at[2 * t * pitch + n * 8 + g], at[(2 * t + 1) * pitch + n * 8 + g]);
   }
 }
+
+// c (sum of the small terms) and ch (sum of the large ones) += a b, a given as hi + lo.  The two sums are kept apart
+// because the tensor unit cuts its sums: each is cut relative to its own size.
+template <bool BEXACT>
+__device__ __forceinline__ void mma_apart(float* ch, float* cl, const float* hi, const float* lo, float2 b) {
+  if (BEXACT) {
+    mma(cl, lo, b.x, b.y);
+    mma(ch, hi, b.x, b.y);
+  } else {
+    float h0, l0, h1, l1;
+    split(b.x, h0, l0);
+    split(b.y, h1, l1);
+    mma(cl, lo, h0, h1);
+    mma(ch, hi, h0, h1);
+    mma(cl, hi, l0, l1);
+  }
+}
+// Values of a (token, column) array of global memory for this warp's two token tiles, in accumulator order; those past the
+// sequence's end or the last column are zero.  row0: the chunk's first token, column g of the group's first.
+template <typename E>
+__device__ __forceinline__ void fetch_own(E (*x)[4], const E* row0, int64_t stride, const int* own, int t, int left, bool in0,
+                                          bool in1) {
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int tok = own[e] * 8 + 2 * t + j;
+      const E* p = row0 + tok * stride;
+      x[e][j] = tok < left && in0 ? p[0] : from_f<E>(0.f);
+      x[e][2 + j] = tok < left && in1 ? p[8] : from_f<E>(0.f);
+    }
+}
+__device__ __forceinline__ void clear(float* c) { c[0] = c[1] = c[2] = c[3] = 0.f; }
 
 __device__ __forceinline__ int row_length(const Args& a, int b) {
   if (!a.lengths) return (int)a.T;
   const int64_t n = a.lengths[b];
   return (int)(n < 0 ? 0 : (n > a.T ? a.T : n));
 }
+
+// Barrier of the four warps of a group.
+__device__ __forceinline__ void group_sync(int grp) { asm volatile("bar.sync %0, 128;" ::"r"(grp + 1) : "memory"); }
+
+int scan_groups(const Args& a, int sms);   // groups of 16 value columns to a block (plastic_scan.cu)
 
 // Launchers (one translation unit per kernel family).
 int launch_prepare(const Args& a, int dtype, bool backward, cudaStream_t st);

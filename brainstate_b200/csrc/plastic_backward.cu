@@ -1,7 +1,7 @@
 // Gated delta rule, reverse mode.
 //
 // backward_scan_kernel: the pass over the chunks from the last to the first that carries the cotangent of the state,
-// in the same register form as the forward pass (16 value columns a group, transposed, accumulators used as left
+// in the same form as the forward pass (groups of 16 value columns, transposed, accumulators used as left
 // operands).  With dS the cotangent of the state after the chunk:
 //   dU = P^T dO + diag(e^{G_C-G}) K dS,  dY = T^T dU,  dV = beta dY,  dR = -beta e^G dY,
 //   dS <- e^{G_C} dS + Q^T (scale e^G dO) + K^T dR.
@@ -23,39 +23,114 @@ namespace plastic {
 
 template <typename E, int DK>
 struct BackScanLayout {
-  static constexpr int PK = DK + 8, PT = kC + 8, PP = kC + 4;   // T^T and P are read by column: PP
+  static constexpr int PK = DK + 8;
   static constexpr size_t tile = (size_t)kC * PK * sizeof(E);
-  static constexpr size_t tri = (size_t)kC * PP * sizeof(float);
-  static constexpr int stages = (sizeof(E) == 4 && DK == 128) ? 1 : 2;
-  static constexpr size_t q_off = tile, t_off = 2 * tile, p_off = t_off + tri, vec_off = p_off + tri,
-                          v_off = vec_off + 3 * kC * sizeof(float);
-  static size_t v_bytes(int groups) { return (size_t)kC * (groups * 16 + 8) * sizeof(E); }
-  static size_t red_bytes(int groups, int ws) { return ws > 1 ? (size_t)groups * ws * 32 * 32 * 4 : 0; }
-  static size_t bytes(int groups, int ws) { return stages * (v_off + v_bytes(groups)) + red_bytes(groups, ws); }
+  static constexpr uint32_t rec = (2 * kTri + 3 * kC) * sizeof(float);
+  static constexpr size_t set = 2 * tile + rec;        // K, Q, record (T, P, vectors)
+  // a group's exchange: dS (then dR and scale e^G dO), dU, dO
+  static constexpr size_t group = 16384 + 8192 + 4096;
+  static constexpr size_t bytes(int groups, int stages) { return stages * set + groups * group; }
 };
 
-template <typename E, int DK, int WS>
-__global__ void __launch_bounds__(256) backward_scan_kernel(Args a, int groups) {
+// The pair (row 2t, row 2t + 1) of column g of a packed 8x8 tile.
+__device__ __forceinline__ float2 column_pair(const float* tile, int lane) {
+  const float* p = tile + (lane & 3) * 16 + (lane >> 2);
+  return make_float2(p[0], p[8]);
+}
+
+// r += dO^T P of token tiles W and 7 - W.
+template <int W, bool X>
+__device__ __forceinline__ void gather_own(const float4* gO, const float* Pm, int lane, float (*r)[4]) {
+  float h[2][4], x[2][4];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    clear(h[e]);
+    clear(x[e]);
+  }
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks) {
+    if (ks < W && ks < 7 - W) continue;
+    const float4 v = gO[ks * 32 + lane];
+    const float c[4] = {v.x, v.y, v.z, v.w};
+    float hi[4], lo[4];
+    if (!X) split4(c, hi, lo);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int n = e ? 7 - W : W;
+      if (ks < n) continue;
+      const float2 pp = column_pair(Pm + tri(ks, n), lane);
+      if (X) {
+        float h0, l0, h1, l1;
+        split(pp.x, h0, l0);
+        split(pp.y, h1, l1);
+        mma(x[e], c, l0, l1);
+        mma(h[e], c, h0, h1);
+      } else {
+        mma_apart<false>(h[e], x[e], hi, lo, pp);
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[e][i] += h[e][i] + x[e][i];
+}
+
+// dY^T = dU^T T of the same token tiles.
+template <int W>
+__device__ __forceinline__ void solve_back_own(const float4* gU, const float* Tm, int lane, float (*y)[4]) {
+  float h[2][4], x[2][4], z[2][4];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    clear(h[e]);
+    clear(x[e]);
+    clear(z[e]);
+  }
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks) {
+    if (ks < W && ks < 7 - W) continue;
+    float hi[4], lo[4];
+    get_split(gU, ks, lane, hi, lo);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int n = e ? 7 - W : W;
+      if (ks < n) continue;
+      const float2 tt = column_pair(Tm + tri(ks, n), lane);
+      float h0, l0, h1, l1;
+      split(tt.x, h0, l0);
+      split(tt.y, h1, l1);
+      mma(x[e], lo, h0, h1);
+      mma(z[e], hi, l0, l1);
+      mma(h[e], hi, h0, h1);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[e][i] = h[e][i] + (x[e][i] + z[e][i]);
+}
+
+template <typename E, int DK, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1) backward_scan_kernel(Args a, int groups, int stages) {
   using L = BackScanLayout<E, DK>;
   constexpr bool X = IsExact<E>::value;
-  constexpr int DKW = DK / WS, NT = DKW / 8, NB = NT < 4 ? NT : 4;
+  constexpr int DKW = DK / 4, NT = DKW / 8;
   extern __shared__ __align__(16) unsigned char smem[];
-  const int tid = threadIdx.x, nthr = blockDim.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int grp = warp / WS, w = warp - grp * WS;
+  __shared__ __align__(8) uint64_t bars[2];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int grp = warp >> 2, w = warp & 3;
   const int per_head = (a.dv + 16 * groups - 1) / (16 * groups);
   const int bh = blockIdx.x / per_head, vb = (blockIdx.x - bh * per_head) * groups * 16;
   const int b = bh / a.Hv, h = bh - b * a.Hv, hk = h / (a.Hv / a.Hk);
   const int len = row_length(a, b), nc = (len + kC - 1) / kC;
-  const int PV = groups * 16 + 8;
-  const size_t set = L::v_off + (size_t)kC * PV * sizeof(E);
-  float* red = reinterpret_cast<float*>(smem + L::stages * set);
+  float4* gS = reinterpret_cast<float4*>(smem + stages * L::set + grp * L::group);   // dS; then dR, scale e^G dO
+  float4* gX = gS + 512;
+  float4* gU = gS + 1024;
+  float4* gO = gU + 512;
   const int d0 = vb + grp * 16 + g;
+  const bool in0 = d0 < a.dv, in1 = d0 + 8 < a.dv;
   const int kb = w * DKW;
-
-  const E* kp = static_cast<const E*>(a.k) + b * a.ks[0] + hk * a.ks[2];
-  const E* qp = static_cast<const E*>(a.q) + b * a.qs[0] + hk * a.qs[2];
-  const int64_t os = (int64_t)a.Hv * a.dv;      // token stride of the outputs and their cotangents
-  const E* dop = static_cast<const E*>(a.dout) + (int64_t)b * a.T * os + (int64_t)h * a.dv + vb;
+  const int own[2] = {w, 7 - w};
 
   float s[NT][4];
 #pragma unroll
@@ -66,46 +141,36 @@ __global__ void __launch_bounds__(256) backward_scan_kernel(Args a, int groups) 
       s[n][i] = (a.dstate && kr < a.dk && d < a.dv) ? a.dstate[((int64_t)bh * a.dk + kr) * a.dv + d] : 0.f;
     }
 
-  auto load = [&](int c, int buf) {
-    unsigned char* base = smem + buf * set;
-    const int64_t t0 = (int64_t)c * kC;
-    const int rows = min(kC, len - c * kC);
-    const int64_t ci = (int64_t)bh * a.NC + c;
-    stage(reinterpret_cast<E*>(base), L::PK, kp + t0 * a.ks[1], a.ks[1], rows, a.dk, DK, a.vec_qk, tid, nthr);
-    stage(reinterpret_cast<E*>(base + L::q_off), L::PK, qp + t0 * a.qs[1], a.qs[1], rows, a.dk, DK, a.vec_qk, tid, nthr);
-    stage_lower(reinterpret_cast<float*>(base + L::t_off), L::PP, a.Tm + ci * kC * kC, tid, nthr);
-    stage_lower(reinterpret_cast<float*>(base + L::p_off), L::PP, a.Pm + ci * kC * kC, tid, nthr);
-    for (int i = tid; i < 3 * kC / 4; i += nthr)
-      cp16(base + L::vec_off + i * 16, a.vec + ci * kVec + i * 4, true);
-    stage(reinterpret_cast<E*>(base + L::v_off), PV, dop + t0 * os, os, rows, min(a.dv - vb, groups * 16), groups * 16,
-          a.vec_do, tid, nthr);
-    cp_commit();
+  if (tid < 2) mbar_init(&bars[tid], 1);
+  __syncthreads();
+  const unsigned char* kq = static_cast<const unsigned char*>(a.kq) + ((int64_t)b * a.Hk + hk) * a.NC * (2 * L::tile);
+  auto load = [&](int c, int buf) {    // one thread
+    unsigned char* base = smem + buf * L::set;
+    mbar_expect_tx(&bars[buf], (uint32_t)L::set);
+    bulk_g2s(base, kq + (int64_t)c * (2 * L::tile), (uint32_t)(2 * L::tile), &bars[buf]);
+    bulk_g2s(base + 2 * L::tile, a.rec + ((int64_t)bh * a.NC + c) * kRecord, L::rec, &bars[buf]);
   };
-
-  if (L::stages == 2 && nc > 0) load(nc - 1, (nc - 1) & 1);
-  for (int c = nc - 1; c >= 0; --c) {
-    const int buf = L::stages == 2 ? (c & 1) : 0;
-    if (L::stages == 2) {
-      if (c > 0) {
-        load(c - 1, buf ^ 1);
-        cp_wait<1>();
-      } else {
-        cp_wait<0>();
-      }
-    } else {
-      load(c, 0);
-      cp_wait<0>();
-    }
-    __syncthreads();
-    const unsigned char* base = smem + buf * set;
+  const int64_t os = (int64_t)a.Hv * a.dv;      // token stride of the outputs and their cotangents
+  const E* dop = static_cast<const E*>(a.dout) + (int64_t)b * a.T * os + (int64_t)h * a.dv + d0;
+  E on[2][4];
+  if (nc > 0) {
+    if (tid == 0) load(nc - 1, 0);
+    fetch_own(on, dop + (int64_t)(nc - 1) * kC * os, os, own, t, len - (nc - 1) * kC, in0, in1);
+  }
+  for (int i = 0; i < nc; ++i) {
+    const int c = nc - 1 - i;
+    const int buf = stages == 2 ? (i & 1) : 0;
+    if (stages == 2 && c > 0 && tid == 0) load(c - 1, buf ^ 1);
+    const bool there = stage_wait(&bars[buf], stages == 2 ? ((i >> 1) & 1) : (i & 1));
+    if (!there) s[0][0] = s[0][1] = s[0][2] = s[0][3] = __int_as_float(0x7fffffff);
+    const unsigned char* base = smem + buf * L::set;
     const E* K = reinterpret_cast<const E*>(base);
-    const E* Q = reinterpret_cast<const E*>(base + L::q_off);
-    const float* Tm = reinterpret_cast<const float*>(base + L::t_off);
-    const float* Pm = reinterpret_cast<const float*>(base + L::p_off);
-    const float* eG = reinterpret_cast<const float*>(base + L::vec_off);
+    const E* Q = reinterpret_cast<const E*>(base + L::tile);
+    const float* Tm = reinterpret_cast<const float*>(base + 2 * L::tile);
+    const float* Pm = Tm + kTri;
+    const float* eG = Pm + kTri;
     const float* eD = eG + kC;
     const float* beta = eG + 2 * kC;
-    const E* DO = reinterpret_cast<const E*>(base + L::v_off) + grp * 16;
     const int64_t ci = (int64_t)bh * a.NC + c;
     const int64_t t0 = (int64_t)c * kC;
 
@@ -119,165 +184,119 @@ __global__ void __launch_bounds__(256) backward_scan_kernel(Args a, int groups) 
             *reinterpret_cast<float2*>(out + (int64_t)(d0 + 8 * hf) * DK + kb + n * 8 + 2 * t) =
                 make_float2(s[n][2 * hf], s[n][2 * hf + 1]);
     }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) put_split(gS, w * NT + n, lane, s[n]);
+    float x[2][4];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[e][j] = to_f<E>(on[e][j]);
+      gO[own[e] * 32 + lane] = make_float4(x[e][0], x[e][2], x[e][1], x[e][3]);
+    }
+    if (c > 0) fetch_own(on, dop + (t0 - kC) * os, os, own, t, kC, in0, in1);
+    group_sync(grp);
 
-    // dS^T K^T over this warp's key rows, scaled by e^{G_C-G}
-    float r[8][4];
+    // dU^T = e^{G_C-G} dS^T K^T + dO^T P of this warp's tokens
+    float rh[2][4], rl[2][4];
 #pragma unroll
-    for (int n = 0; n < 8; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) r[n][i] = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < NT; ++ks) {
-      float x[4], hi[4], lo[4];
-      as_left(s[ks], x);
-      split4(x, hi, lo);
-      float2 kk[8];
-#pragma unroll
-      for (int n = 0; n < 8; ++n) kk[n] = pair(K + (n * 8 + g) * L::PK + kb + ks * 8 + 2 * t);
-      mma_split<X, 8>(r, hi, lo, kk);
+    for (int e = 0; e < 2; ++e) {
+      clear(rh[e]);
+      clear(rl[e]);
     }
-    if (WS > 1) {
-      float* mine = red + (size_t)grp * WS * 32 * 32 + lane;   // free since the barrier at the chunk's end
+#pragma unroll 4
+    for (int ks = 0; ks < DK / 8; ++ks) {
+      float hi[4], lo[4];
+      get_split(gS, ks, lane, hi, lo);
 #pragma unroll
-      for (int n = 0; n < 8; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mine[(w * 32 + n * 4 + i) * 32] = r[n][i];
-      asm volatile("bar.sync %0, %1;" ::"r"(grp + 1), "n"(WS * 32) : "memory");
-#pragma unroll
-      for (int n = 0; n < 8; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float x = mine[(n * 4 + i) * 32];
-#pragma unroll
-          for (int p = 1; p < WS; ++p) x += mine[(p * 32 + n * 4 + i) * 32];
-          r[n][i] = x;
-        }
+      for (int e = 0; e < 2; ++e)
+        mma_apart<X>(rh[e], rl[e], hi, lo, pair(K + (own[e] * 8 + g) * L::PK + ks * 8 + 2 * t));
     }
 #pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      const float2 ed = pair(eD + n * 8 + 2 * t);
-      r[n][0] *= ed.x;
-      r[n][1] *= ed.y;
-      r[n][2] *= ed.x;
-      r[n][3] *= ed.y;
-    }
-    // dO^T (value columns as rows), then dU^T = dO^T P + ...
-    float x[8][4];
+    for (int e = 0; e < 2; ++e) {
+      const float2 ed = pair(eD + own[e] * 8 + 2 * t);
 #pragma unroll
-    for (int n = 0; n < 8; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[n][i] = to_f<E>(DO[(n * 8 + 2 * t + (i & 1)) * PV + g + 8 * (i >> 1)]);
-#pragma unroll
-    for (int ks = 0; ks < 8; ++ks) {
-      float y[4], hi[4], lo[4];
-      as_left(x[ks], y);
-      if (!X) split4(y, hi, lo);
-      float2 ph[8], pl[8];
-#pragma unroll
-      for (int n = 0; n <= ks; ++n) {
-        const float* p = Pm + (ks * 8 + 2 * t) * L::PP + n * 8 + g;
-        split(p[0], ph[n].x, pl[n].x);
-        split(p[L::PP], ph[n].y, pl[n].y);
-      }
-      if (X) {
-#pragma unroll
-        for (int n = 0; n <= ks; ++n) mma(r[n], y, pl[n].x, pl[n].y);
-#pragma unroll
-        for (int n = 0; n <= ks; ++n) mma(r[n], y, ph[n].x, ph[n].y);
-      } else {
-#pragma unroll
-        for (int n = 0; n <= ks; ++n) mma(r[n], lo, ph[n].x, ph[n].y);
-#pragma unroll
-        for (int n = 0; n <= ks; ++n) mma(r[n], hi, pl[n].x, pl[n].y);
-#pragma unroll
-        for (int n = 0; n <= ks; ++n) mma(r[n], hi, ph[n].x, ph[n].y);
+      for (int j = 0; j < 4; ++j) {
+        const float f = (j & 1) ? ed.y : ed.x;
+        rh[e][j] *= f;
+        rl[e][j] *= f;
       }
     }
-    // dY^T = dU^T T
-    float dy[8][4];
+    float u[2][4], y[2][4];
 #pragma unroll
-    for (int n = 0; n < 8; ++n)
+    for (int e = 0; e < 2; ++e)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) dy[n][i] = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < 8; ++ks) {
-      float y[4], hi[4], lo[4];
-      as_left(r[ks], y);
-      split4(y, hi, lo);
-      float2 th[8], tl[8];
-#pragma unroll
-      for (int n = 0; n <= ks; ++n) {
-        const float* p = Tm + (ks * 8 + 2 * t) * L::PP + n * 8 + g;
-        split(p[0], th[n].x, tl[n].x);
-        split(p[L::PP], th[n].y, tl[n].y);
-      }
-#pragma unroll
-      for (int n = 0; n <= ks; ++n) mma(dy[n], lo, th[n].x, th[n].y);
-#pragma unroll
-      for (int n = 0; n <= ks; ++n) mma(dy[n], hi, tl[n].x, tl[n].y);
-#pragma unroll
-      for (int n = 0; n <= ks; ++n) mma(dy[n], hi, th[n].x, th[n].y);
+      for (int j = 0; j < 4; ++j) u[e][j] = rh[e][j] + rl[e][j];
+    switch (w) {
+      case 0: gather_own<0, X>(gO, Pm, lane, u); break;
+      case 1: gather_own<1, X>(gO, Pm, lane, u); break;
+      case 2: gather_own<2, X>(gO, Pm, lane, u); break;
+      default: gather_own<3, X>(gO, Pm, lane, u);
     }
-    if (w == 0) {
-      float* Y = a.dY + ci * a.dv * kC;
-      E* dv = static_cast<E*>(a.dv_) + ((int64_t)b * a.T + t0) * os + (int64_t)h * a.dv;
 #pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        const int tok = n * 8 + 2 * t;
-        const float2 be = pair(beta + tok);
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          const int d = d0 + 8 * hf;
-          if (d >= a.dv) continue;
-          *reinterpret_cast<float2*>(Y + (int64_t)d * kC + tok) = make_float2(dy[n][2 * hf], dy[n][2 * hf + 1]);
-          if (t0 + tok < len) dv[tok * os + d] = from_f<E>(be.x * dy[n][2 * hf]);
-          if (t0 + tok + 1 < len) dv[(tok + 1) * os + d] = from_f<E>(be.y * dy[n][2 * hf + 1]);
-        }
-      }
+    for (int e = 0; e < 2; ++e) put_split(gU, own[e], lane, u[e]);
+    group_sync(grp);
+
+    switch (w) {
+      case 0: solve_back_own<0>(gU, Tm, lane, y); break;
+      case 1: solve_back_own<1>(gU, Tm, lane, y); break;
+      case 2: solve_back_own<2>(gU, Tm, lane, y); break;
+      default: solve_back_own<3>(gU, Tm, lane, y);
     }
-    // dR^T and scale e^G dO^T as left operands of the state's cotangent
+    float* Y = a.dY + ci * a.dv * kC;
+    E* dv = static_cast<E*>(a.dv_) + ((int64_t)b * a.T + t0) * os + (int64_t)h * a.dv + d0;
 #pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      const int tok = n * 8 + 2 * t;
+    for (int e = 0; e < 2; ++e) {
+      const int tok = own[e] * 8 + 2 * t;
       const float2 be = pair(beta + tok), eg = pair(eG + tok);
+      if (in0) *reinterpret_cast<float2*>(Y + (int64_t)d0 * kC + tok) = make_float2(y[e][0], y[e][1]);
+      if (in1) *reinterpret_cast<float2*>(Y + (int64_t)(d0 + 8) * kC + tok) = make_float2(y[e][2], y[e][3]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float e = (i & 1) ? eg.y : eg.x, bb = (i & 1) ? be.y : be.x;
-        dy[n][i] *= -e * bb;
-        x[n][i] *= a.scale * e;
+      for (int j = 0; j < 2; ++j) {
+        E* o = dv + (tok + j) * os;
+        const float bj = j ? be.y : be.x;
+        if (tok + j < len - c * kC) {
+          if (in0) o[0] = from_f<E>(bj * y[e][j]);
+          if (in1) o[8] = from_f<E>(bj * y[e][2 + j]);
+        }
       }
+      // dR^T and scale e^G dO^T: left operands of the state's cotangent
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float f = (j & 1) ? eg.y : eg.x;
+        y[e][j] *= -f * ((j & 1) ? be.y : be.x);
+        x[e][j] *= a.scale * f;
+      }
+      put_split(gS, own[e], lane, y[e]);
+      put_split(gX, own[e], lane, x[e]);
+    }
+    group_sync(grp);
+
+    float ah[NT][4], al[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      clear(ah[n]);
+      clear(al[n]);
+    }
+#pragma unroll 2
+    for (int ks = 0; ks < 8; ++ks) {
+      float hi[4], lo[4];
+      float2 kk[NT];
+      get_split(gS, ks, lane, hi, lo);
+      tiles_by_row<NT>(kk, K + ks * 8 * L::PK + kb, L::PK, lane);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mma_apart<X>(ah[n], al[n], hi, lo, kk[n]);
+      get_split(gX, ks, lane, hi, lo);
+      tiles_by_row<NT>(kk, Q + ks * 8 * L::PK + kb, L::PK, lane);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mma_apart<X>(ah[n], al[n], hi, lo, kk[n]);
     }
     const float eC = eG[kC - 1];
 #pragma unroll
-    for (int n0 = 0; n0 < NT; n0 += NB) {
-      float acc[NB][4];
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < 8; ++ks) {
-        float y[4], hi[4], lo[4], hi2[4], lo2[4];
-        as_left(dy[ks], y);
-        split4(y, hi, lo);
-        as_left(x[ks], y);
-        split4(y, hi2, lo2);
-        float2 kk[NB], qq[NB];
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          const int at = (ks * 8 + 2 * t) * L::PK + kb + (n0 + n) * 8 + g;
-          kk[n] = make_float2(to_f<E>(K[at]), to_f<E>(K[at + L::PK]));
-          qq[n] = make_float2(to_f<E>(Q[at]), to_f<E>(Q[at + L::PK]));
-        }
-        mma_split<X, NB>(acc, hi, lo, kk);
-        mma_split<X, NB>(acc, hi2, lo2, qq);
-      }
-#pragma unroll
-      for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[n0 + n][i] = fmaf(eC, s[n0 + n][i], acc[n][i]);
-    }
-    __syncthreads();
+      for (int j = 0; j < 4; ++j) s[n][j] = fmaf(eC, s[n][j], ah[n][j] + al[n][j]);
+    __syncthreads();      // the tiles and the group's exchange are free
+    if (stages == 1 && c > 0 && tid == 0) load(c - 1, 0);
   }
   if (a.dinitial) {
 #pragma unroll
@@ -290,32 +309,26 @@ __global__ void __launch_bounds__(256) backward_scan_kernel(Args a, int groups) 
   }
 }
 
-template <typename E, int DK, int WS>
-static int launch_scan_one(const Args& a, int groups, cudaStream_t st) {
-  const size_t bytes = BackScanLayout<E, DK>::bytes(groups, WS);
+template <typename E, int DK, int THREADS>
+static int launch_scan_threads(const Args& a, int groups, cudaStream_t st) {
+  using L = BackScanLayout<E, DK>;
   static std::atomic<uint64_t> seen;
-  int rc = allow_smem(backward_scan_kernel<E, DK, WS>, kMaxSmem, seen);
+  int rc = allow_smem(backward_scan_kernel<E, DK, THREADS>, kMaxSmem, seen);
   if (rc != BSX_OK) return rc;
+  const int stages = L::bytes(groups, 2) <= kMaxSmem ? 2 : 1;
   const int per_head = (a.dv + 16 * groups - 1) / (16 * groups);
   const unsigned grid = (unsigned)((int64_t)a.B * a.Hv * per_head);
-  backward_scan_kernel<E, DK, WS><<<grid, groups * WS * 32, bytes, st>>>(a, groups);
+  backward_scan_kernel<E, DK, THREADS><<<grid, groups * 128, L::bytes(groups, stages), st>>>(a, groups, stages);
   BSX_LAUNCH_CHECK("plastic backward_scan_kernel");
   return BSX_OK;
 }
 
 template <typename E, int DK>
 static int launch_scan_typed(const Args& a, cudaStream_t st) {
-  const int64_t total = (int64_t)a.B * a.Hv * ((a.dv + 15) / 16);
-  const int most = (a.dv + 15) / 16;
   const int sms = sm_count();
   if (sms <= 0) return fail(BSX_ERR_CUDA, "no CUDA device");
-  const int ws = total <= 2 * (int64_t)sms ? 4 : (total <= 4 * (int64_t)sms ? 2 : 1);   // as in the forward pass
-  int groups = ws == 4 ? 1 : 4;
-  while (groups > most) groups >>= 1;
-  while (groups > 1 && BackScanLayout<E, DK>::bytes(groups, ws) > kMaxSmem) groups >>= 1;
-  if (ws == 4) return launch_scan_one<E, DK, 4>(a, groups, st);
-  if (ws == 2) return launch_scan_one<E, DK, 2>(a, groups, st);
-  return launch_scan_one<E, DK, 1>(a, groups, st);
+  const int groups = scan_groups(a, sms);
+  return groups == 4 ? launch_scan_threads<E, DK, 512>(a, groups, st) : launch_scan_threads<E, DK, 256>(a, groups, st);
 }
 
 // ------------------------------------------------------------------------------------------------ all chunks at once
@@ -370,11 +383,11 @@ __global__ void __launch_bounds__(256) backward_chunk_kernel(Args a) {
   const int rows = (int)min((int64_t)kC, len - t0);
   const int64_t ci = (int64_t)bh * a.NC + chunk;
 
-  stage(K, L::PK, static_cast<const E*>(a.k) + b * a.ks[0] + t0 * a.ks[1] + hk * a.ks[2], a.ks[1], rows, a.dk, DK,
-        a.vec_qk, tid, 256);
-  stage(Q, L::PK, static_cast<const E*>(a.q) + b * a.qs[0] + t0 * a.qs[1] + hk * a.qs[2], a.qs[1], rows, a.dk, DK,
-        a.vec_qk, tid, 256);
-  for (int i = tid; i < kVec / 4; i += 256) cp16(eG + i * 4, a.vec + ci * kVec + i * 4, true);
+  {
+    const int4* kq = static_cast<const int4*>(a.kq) + (((int64_t)b * a.Hk + hk) * a.NC + chunk) * (2 * L::tile / 16);
+    for (int i = tid; i < (int)(2 * L::tile / 16); i += 256) cp16(reinterpret_cast<int4*>(smem) + i, kq + i, true);
+  }
+  for (int i = tid; i < kVec / 4; i += 256) cp16(eG + i * 4, a.rec + ci * kRecord + 2 * kTri + i * 4, true);
   cp_commit();
 
   float d1[2][NC4][4], dqa[2][NC4][4], d3[2][NC4][4], dp[2][2][4], da[2][2][4];
@@ -541,8 +554,8 @@ __global__ void __launch_bounds__(256) backward_chunk_kernel(Args a) {
   // E, F and the sums of dP P + dA A, dA (A/beta)
   float* sE = F + L::e;
   float* sF = F + L::f;
-  const float* Pm = a.Pm + ci * kC * kC;
-  const float* Bm = a.Bm + ci * kC * kC;
+  const float* Pm = a.rec + ci * kRecord + kTri;
+  const float* Bm = a.Bm + ci * kTri;
   float cs[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
   float bsum[4];
 #pragma unroll
@@ -558,11 +571,12 @@ __global__ void __launch_bounds__(256) backward_chunk_kernel(Args a) {
         if (j <= i) {
           const float gam = expf((gHi[i] - gHi[j]) + (gLo[i] - gLo[j]));
           const float dpv = dp[r >> 1][n][2 * (r & 1) + e];
-          float m = dpv * Pm[i * kC + j];
+          const int at = tri(i >> 3, j >> 3) + (i & 7) * 8 + (j & 7);
+          float m = dpv * Pm[at];
           ev = a.scale * gam * dpv;
           if (j < i) {
             const float dav = -da[r >> 1][n][2 * (r & 1) + e];
-            const float nb = dav * Bm[i * kC + j];
+            const float nb = dav * Bm[at];
             bsr += nb;
             m = fmaf(beta[i], nb, m);
             fv = beta[i] * gam * dav;

@@ -1,6 +1,7 @@
 // Gated delta rule: what a chunk needs that does not depend on the state — T, P and the decay vectors — for all
 // chunks at once, one block of four warps per (row, head, chunk).
 //
+// The K and Q tiles are also written back in the layout they have in shared memory, once per key head.
 // K K^T and Q K^T are 64x64xdk products (only the tiles on and below the diagonal); T = (I + A)^{-1} is built by
 // substitution: the four 16x16 diagonal blocks by columns (one lane each), then
 // T_ij = -T_ii sum_l A_il T_lj by block distance, in 32-bit arithmetic.  (A power series would need fewer steps but
@@ -69,7 +70,7 @@ __global__ void __launch_bounds__(128) prepare_kernel(Args a) {
     }
     const double G1 = s, G0 = s - x1, GC = __shfl_sync(0xffffffffu, s, 31);
     // s - x1 is not the sum in order, but within 2^-52 of it
-    float* vec = a.vec + ci * kVec;
+    float* vec = a.rec + ci * kRecord + 2 * kTri;
     const float h0 = (float)G0, h1 = (float)G1;
     const float l0 = (float)(G0 - h0), l1 = (float)(G1 - h1);
     sHi[2 * lane] = h0; sHi[2 * lane + 1] = h1;
@@ -83,6 +84,10 @@ __global__ void __launch_bounds__(128) prepare_kernel(Args a) {
   }
   cp_wait<0>();
   __syncthreads();
+  if (h % (a.Hv / a.Hk) == 0) {   // both tiles as they lie here: later kernels take them with one copy
+    int4* kq = static_cast<int4*>(a.kq) + (((int64_t)b * a.Hk + hk) * a.NC + chunk) * (2 * L::tile / 16);
+    for (int i = tid; i < (int)(2 * L::tile / 16); i += 128) kq[i] = reinterpret_cast<const int4*>(smem)[i];
+  }
 
   // rows 16 * warp .. + 15 of K K^T and Q K^T, tiles on and below the diagonal
   float kk[8][4], qk[8][4];
@@ -119,8 +124,9 @@ __global__ void __launch_bounds__(128) prepare_kernel(Args a) {
       }
     }
   }
-  float* Pm = a.Pm + ci * (kC * kC);
-  float* Bm = BACK ? a.Bm + ci * (kC * kC) : nullptr;
+  float* Tm = a.rec + ci * kRecord;
+  float* Pm = Tm + kTri;
+  float* Bm = BACK ? a.Bm + ci * kTri : nullptr;
 #pragma unroll
   for (int n = 0; n < 8; ++n) {
     if (n > 2 * warp + 1) break;
@@ -135,8 +141,11 @@ __global__ void __launch_bounds__(128) prepare_kernel(Args a) {
         m[e] = j + e < i ? gam * kk[n][2 * hf + e] : 0.f;
         sA[i * L::PA + j + e] = sBeta[i] * m[e];
       }
-      *reinterpret_cast<float2*>(Pm + i * kC + j) = make_float2(p[0], p[1]);
-      if (BACK) *reinterpret_cast<float2*>(Bm + i * kC + j) = make_float2(m[0], m[1]);
+      if (n <= 2 * warp + hf) {
+        const int at = tri(2 * warp + hf, n) + lane * 2;
+        *reinterpret_cast<float2*>(Pm + at) = make_float2(p[0], p[1]);
+        if (BACK) *reinterpret_cast<float2*>(Bm + at) = make_float2(m[0], m[1]);
+      }
     }
   }
   __syncthreads();
@@ -174,11 +183,11 @@ __global__ void __launch_bounds__(128) prepare_kernel(Args a) {
     }
     __syncthreads();
   }
-  float* Tm = a.Tm + ci * (kC * kC);
-  for (int e = tid; e < kC * kC; e += 128) {
-    const int r = e >> 6, c = e & 63;
-    if (c < ((r >> 4) + 1) * 16) Tm[e] = sT[r * L::PA + c];
-  }
+  for (int n = warp; n < 8; n += 4)
+    for (int k = 0; k <= n; ++k) {
+      const float* x = sT + (n * 8 + g) * L::PA + k * 8 + 2 * t;
+      *reinterpret_cast<float2*>(Tm + tri(n, k) + lane * 2) = make_float2(x[0], x[1]);
+    }
 }
 
 template <typename E, int DK>

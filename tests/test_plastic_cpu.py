@@ -41,8 +41,8 @@ def test_library_refusals_need_no_gpu(bsx):
     assert fwd(_desc(batch=0)) == 0 and bsx.bsx_delta_recurrent(C.byref(_desc(batch=0)), None, None, None) == 0
     assert bsx.bsx_delta_backward(C.byref(_desc(**full)), None, None, None, None, None, None, None, None, None, 0,
                                   None) == BSX_ERR_INVALID_ARG
-    # two chunks of two heads of two rows: T, P and the vectors; reverse mode more
-    assert bsx.bsx_delta_workspace_bytes(C.byref(_desc())) == 2 * 2 * 2 * (2 * 4096 + 320) * 4
+    # at least T and P of two chunks of two heads of two rows; reverse mode needs more
+    assert bsx.bsx_delta_workspace_bytes(C.byref(_desc())) >= 2 * 2 * 2 * 2 * 36 * 64 * 4
     assert bsx.bsx_delta_backward_workspace_bytes(C.byref(_desc())) > bsx.bsx_delta_workspace_bytes(C.byref(_desc()))
     assert bsx.bsx_delta_workspace_bytes(C.byref(_desc(dk=500))) == 0
 
