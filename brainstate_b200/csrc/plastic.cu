@@ -14,7 +14,7 @@ static size_t workspace(const bsx_delta_t* d, bool backward) {
   const size_t size = d->dtype == BSX_T_F32 ? 4 : 2;
   size_t f = (size_t)n * kRecord + (size_t)(n / (d->v_heads / d->k_heads)) * (2 * kC * (width_of(d->dk) + 8) * size / 4);
   if (backward) {
-    f += (size_t)n * (kTri + 2 * (size_t)d->dv * (width_of(d->dk) + kC));
+    f += (size_t)n * (kTri + 2 * (size_t)d->dv * (width_of(d->dk) + 4 + kPU));
     if (d->k_heads != d->v_heads) f += 2 * (size_t)d->batch * d->tokens * d->v_heads * d->dk;
   }
   return f * sizeof(float);
@@ -73,12 +73,12 @@ static void place(Args& a, const bsx_delta_t* d, float* ws, bool backward) {
   a.kq = ws; ws += (int64_t)a.B * a.Hk * a.NC * (2 * kC * (width_of(a.dk) + 8) * (d->dtype == BSX_T_F32 ? 4 : 2) / 4);
   a.rec = ws; ws += n * kRecord;
   if (!backward) return;
-  const int64_t wide = width_of(a.dk);
+  const int64_t wide = width_of(a.dk) + 4;
   a.Bm = ws; ws += n * kTri;
   a.Sn = ws; ws += n * a.dv * wide;
   a.dS = ws; ws += n * a.dv * wide;
-  a.U = ws; ws += n * a.dv * kC;
-  a.dY = ws; ws += n * a.dv * kC;
+  a.U = ws; ws += n * a.dv * kPU;
+  a.dY = ws; ws += n * a.dv * kPU;
   if (a.Hk != a.Hv) {
     a.dq32 = ws; ws += (int64_t)a.B * a.T * a.Hv * a.dk;
     a.dk32 = ws;

@@ -41,7 +41,8 @@ struct Args {
   void* kq;
   // per (row, value head, chunk): T, P and vectors (kRecord floats); A / beta (kTri), backward only
   float *rec, *Bm;
-  // per (row, head, chunk), transposed: state before the chunk (dv, DK), U (dv, 64); backward only
+  // per (row, head, chunk), transposed: state before the chunk (dv rows of DK + 4), U (dv rows of 68); backward only.  The
+  // rows lie as in shared memory, so that a block of them is one copy; dS (after the chunk) and dY likewise
   float *Sn, *U;
   void* o;
   float* state;
@@ -54,6 +55,8 @@ struct Args {
   float *dq32, *dk32;     // per value head, when heads share keys
   bool vec_qk;            // rows of q and k start on 16-byte boundaries and are whole 16-byte stretches
 };
+
+constexpr int kPU = kC + 4;
 
 template <typename E> __device__ __forceinline__ float to_f(E x);
 template <> __device__ __forceinline__ float to_f<float>(float x) { return x; }
@@ -179,18 +182,18 @@ __device__ __forceinline__ bool stage_wait(uint64_t* bar, uint32_t parity) {
   return false;
 }
 
-// Operand tiles (16 value columns x 8) handed from one warp of a group to the others, already split: 1 KB a tile, in
-// the order of a left operand's registers.
+// Operand tiles (16 value columns x 8) handed from one warp of a group to the others, already split: 1 KB a tile, the
+// four registers of the left operand together (anything else costs moves).
 __device__ __forceinline__ void put_split(float4* base, int tile, int lane, const float* c) {
   float h[4], l[4];
   split4(c, h, l);
-  base[tile * 64 + lane] = make_float4(h[0], l[0], h[2], l[2]);
-  base[tile * 64 + 32 + lane] = make_float4(h[1], l[1], h[3], l[3]);
+  base[tile * 64 + lane] = make_float4(h[0], h[2], h[1], h[3]);
+  base[tile * 64 + 32 + lane] = make_float4(l[0], l[2], l[1], l[3]);
 }
 __device__ __forceinline__ void get_split(const float4* base, int tile, int lane, float* hi, float* lo) {
   const float4 x = base[tile * 64 + lane], y = base[tile * 64 + 32 + lane];
-  hi[0] = x.x; lo[0] = x.y; hi[1] = x.z; lo[1] = x.w;
-  hi[2] = y.x; lo[2] = y.y; hi[3] = y.z; lo[3] = y.w;
+  hi[0] = x.x; hi[1] = x.y; hi[2] = x.z; hi[3] = x.w;
+  lo[0] = y.x; lo[1] = y.y; lo[2] = y.z; lo[3] = y.w;
 }
 
 // Right-operand tiles from a (row, column) tile in shared memory: N 8x8 tiles whose rows are the outer index (pairs of
@@ -210,8 +213,10 @@ __device__ __forceinline__ void tiles_by_row(float2* b, const E* at, int pitch, 
     if constexpr (N == 4)
       asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                    : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-    else
+    else if constexpr (N == 2)
       asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
+    else
+      asm volatile("ldmatrix.sync.aligned.m8n8.x1.trans.shared.b16 {%0}, [%1];" : "=r"(r[0]) : "r"(addr) : "memory");
 #pragma unroll
     for (int n = 0; n < N; ++n) b[n] = unpack(r[n], at);
   } else {

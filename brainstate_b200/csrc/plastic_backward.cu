@@ -7,8 +7,8 @@
 //   dS <- e^{G_C} dS + Q^T (scale e^G dO) + K^T dR.
 // It leaves dS (before the update) and dY for every chunk.
 //
-// backward_chunk_kernel: everything else, all chunks at once, one block per (row, head, chunk).  Over blocks of 32 value
-// columns it sums D1 = dY S0^T, Dq = dO S0^T, D3 = U dS^T (64 x dk) and dP = dO U^T, dA = -dY U^T (64 x 64), then
+// backward_chunk_kernel: everything else, all chunks at once, one block of 16 warps per (row, head, chunk).  Over blocks of 32
+// value columns (bulk copies, one block ahead) it sums D1 = dY S0^T, Dq = dO S0^T, D3 = U dS^T (64 x dk) and dP = dO U^T, dA = -dY U^T (64 x 64), then
 //   dQ = scale e^G Dq + E K,                         E = scale Gamma dP (j <= i)
 //   dK = -beta e^G D1 + e^{G_C-G} D3 + E^T Q + (F + F^T) K,   F = beta Gamma dA (j < i)
 //   dbeta_i = dY_i.V_i - e^{G_i} K_i.D1_i + sum_j dA_ij (A/beta)_ij
@@ -175,13 +175,13 @@ __global__ void __launch_bounds__(THREADS, 1) backward_scan_kernel(Args a, int g
     const int64_t t0 = (int64_t)c * kC;
 
     {
-      float* out = a.dS + ci * a.dv * DK;
+      float* out = a.dS + ci * a.dv * (DK + 4);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf)
           if (d0 + 8 * hf < a.dv)
-            *reinterpret_cast<float2*>(out + (int64_t)(d0 + 8 * hf) * DK + kb + n * 8 + 2 * t) =
+            *reinterpret_cast<float2*>(out + (d0 + 8 * hf) * (DK + 4) + kb + n * 8 + 2 * t) =
                 make_float2(s[n][2 * hf], s[n][2 * hf + 1]);
     }
 #pragma unroll
@@ -242,14 +242,14 @@ __global__ void __launch_bounds__(THREADS, 1) backward_scan_kernel(Args a, int g
       case 2: solve_back_own<2>(gU, Tm, lane, y); break;
       default: solve_back_own<3>(gU, Tm, lane, y);
     }
-    float* Y = a.dY + ci * a.dv * kC;
+    float* Y = a.dY + ci * a.dv * kPU;
     E* dv = static_cast<E*>(a.dv_) + ((int64_t)b * a.T + t0) * os + (int64_t)h * a.dv + d0;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int tok = own[e] * 8 + 2 * t;
       const float2 be = pair(beta + tok), eg = pair(eG + tok);
-      if (in0) *reinterpret_cast<float2*>(Y + (int64_t)d0 * kC + tok) = make_float2(y[e][0], y[e][1]);
-      if (in1) *reinterpret_cast<float2*>(Y + (int64_t)(d0 + 8) * kC + tok) = make_float2(y[e][2], y[e][3]);
+      if (in0) *reinterpret_cast<float2*>(Y + d0 * kPU + tok) = make_float2(y[e][0], y[e][1]);
+      if (in1) *reinterpret_cast<float2*>(Y + (d0 + 8) * kPU + tok) = make_float2(y[e][2], y[e][3]);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         E* o = dv + (tok + j) * os;
@@ -334,47 +334,94 @@ static int launch_scan_typed(const Args& a, cudaStream_t st) {
 // ------------------------------------------------------------------------------------------------ all chunks at once
 
 constexpr int kVB = 32;   // value columns of a block
+constexpr int kChunkThreads = 512;
 
 template <typename E, int DK>
 struct BackChunkLayout {
-  static constexpr int PK = DK + 8, PS = DK + 4, PY = kC + 4, PO = kVB + 8, PE = kC + 8;
+  static constexpr int PK = DK + 8, PS = DK + 4, PO = kVB + 8, PE = kC + 8;
   static constexpr size_t tile = (size_t)kC * PK * sizeof(E);
+  // floats of one set of block buffers: S0, dS, U, dY
+  static constexpr int ds = kVB * PS, u = 2 * kVB * PS, dy = u + kVB * kPU, set = dy + kVB * kPU;
   // floats after the K and Q tiles
-  static constexpr int s0 = 0, ds = s0 + kVB * PS, u = ds + kVB * PS, dy = u + kVB * PY, dof = dy + kVB * PY,
-                       vf = dof + kC * PO, loop_end = vf + kC * PO;
-  static constexpr int e = 0, f = kC * PE, tail_end = 2 * kC * PE;       // reuse the block buffers
-  static constexpr int small = loop_end > tail_end ? loop_end : tail_end;
-  static constexpr int vecs = small, parts = vecs + kVec, end = parts + 20 * kC + 8;
+  static constexpr int dof = 2 * set, vecs = dof + kC * PO, parts = vecs + kVec, end = parts + 36 * kC;
+  static constexpr int e = 0, f = kC * PE;       // reuse the block buffers
+  static_assert(2 * kC * PE <= 2 * set, "");
   static constexpr size_t bytes = 2 * tile + (size_t)end * sizeof(float);
 };
 
+// t[m][n] += a b over the four 8-column steps of a block: a (32 rows of this warp, two tiles) from a transposed (column,
+// row) array or, with ROWS, from a (row, column) one; b from two (column, outer) arrays, N tiles of the first and one of
+// the second.  All in 32 bits except a where AEXACT.
+template <bool AEXACT, bool ROWS, int N, bool SECOND>
+__device__ __forceinline__ void block_products(float (*t1)[N][4], float (*t2)[4], const float* a, int pa, const float* b1, int p1,
+                                               const float* b2, int p2, int g, int t) {
+#pragma unroll
+  for (int ks = 0; ks < kVB / 8; ++ks) {
+    const int v = ks * 8 + 2 * t;
+    float hi[2][4], lo[2][4];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      float x[4];
+      if (ROWS) {
+        const float2 p0 = pair(a + (m * 16 + g) * pa + v), q0 = pair(a + (m * 16 + g + 8) * pa + v);
+        x[0] = p0.x; x[1] = q0.x; x[2] = p0.y; x[3] = q0.y;
+      } else {
+        const float* p = a + v * pa + m * 16 + g;
+        x[0] = p[0]; x[1] = p[8]; x[2] = p[pa]; x[3] = p[pa + 8];
+      }
+      if (AEXACT) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) hi[m][i] = x[i];
+      } else {
+        split4(x, hi[m], lo[m]);
+      }
+    }
+    float2 h[N + 1], l[N + 1];
+#pragma unroll
+    for (int n = 0; n < N + (SECOND ? 1 : 0); ++n) {
+      const float* p = n < N ? b1 + v * p1 + n * 8 + g : b2 + v * p2 + g;
+      split(p[0], h[n].x, l[n].x);
+      split(p[n < N ? p1 : p2], h[n].y, l[n].y);
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+#pragma unroll
+      for (int n = 0; n < N + (SECOND ? 1 : 0); ++n) {
+        float* c = n < N ? t1[m][n < N ? n : 0] : t2[m];
+        if (!AEXACT) mma(c, lo[m], h[n].x, h[n].y);
+      }
+#pragma unroll
+      for (int n = 0; n < N + (SECOND ? 1 : 0); ++n) mma(n < N ? t1[m][n < N ? n : 0] : t2[m], hi[m], l[n].x, l[n].y);
+#pragma unroll
+      for (int n = 0; n < N + (SECOND ? 1 : 0); ++n) mma(n < N ? t1[m][n < N ? n : 0] : t2[m], hi[m], h[n].x, h[n].y);
+    }
+  }
+}
+
 template <typename E, int DK>
-__global__ void __launch_bounds__(256) backward_chunk_kernel(Args a) {
+__global__ void __launch_bounds__(kChunkThreads, 1) backward_chunk_kernel(Args a) {
   using L = BackChunkLayout<E, DK>;
   constexpr bool X = IsExact<E>::value;
   constexpr bool SHORT = IsShort<E>::value;
-  constexpr int NC4 = DK / 32;    // 8-wide column tiles of a warp in the (64, DK) products
+  constexpr int N = DK / 64;    // 8-wide column tiles of a warp in the (64, DK) products
+  constexpr int kT = kChunkThreads;
   extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ __align__(8) uint64_t bars[3];
   E* K = reinterpret_cast<E*>(smem);
   E* Q = reinterpret_cast<E*>(smem + L::tile);
   float* F = reinterpret_cast<float*>(smem + 2 * L::tile);
-  float* sS0 = F + L::s0;
-  float* sDS = F + L::ds;
-  float* sU = F + L::u;
-  float* sDY = F + L::dy;
   float* sDO = F + L::dof;
-  float* sV = F + L::vf;
   float* eG = F + L::vecs;
   float* eD = eG + kC;
   float* beta = eG + 2 * kC;
   float* gHi = eG + 3 * kC;
   float* gLo = eG + 4 * kC;
-  // parts: [0,4) row sums of dP P + dA A, [4,6) their column sums, [6,10) K.D1, [10,14) Q.Dq, [14,18) K.D3,
-  //        18 dY.V, 19 row sums of dA (A/beta) by column quarter come in [0,4) of a second use
+  // sums by column eighth, then added: [0,8) rows of dP P + dA A (later dA A/beta), [8,10) its columns, [10,18) K.D1,
+  // [18,26) Q.Dq, [26,34) K.D3, 34 dY.V, 35 <S0,dS>
   float* parts = F + L::parts;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int wr = warp & 1, wc = warp >> 1;     // rows 32 wr .. + 31; columns by quarter wc
+  const int wr = warp & 1, wc = warp >> 1;     // rows 32 wr .. + 31; column eighth wc
   const int chunk = blockIdx.x % a.NC;
   const int bh = blockIdx.x / a.NC, b = bh / a.Hv, h = bh - b * a.Hv, hk = h / (a.Hv / a.Hk);
   const int len = row_length(a, b);
@@ -383,149 +430,135 @@ __global__ void __launch_bounds__(256) backward_chunk_kernel(Args a) {
   const int rows = (int)min((int64_t)kC, len - t0);
   const int64_t ci = (int64_t)bh * a.NC + chunk;
 
-  {
-    const int4* kq = static_cast<const int4*>(a.kq) + (((int64_t)b * a.Hk + hk) * a.NC + chunk) * (2 * L::tile / 16);
-    for (int i = tid; i < (int)(2 * L::tile / 16); i += 256) cp16(reinterpret_cast<int4*>(smem) + i, kq + i, true);
+  const float* gS = a.Sn + ci * a.dv * L::PS;
+  const float* gDS = a.dS + ci * a.dv * L::PS;
+  const float* gU = a.U + ci * a.dv * kPU;
+  const float* gY = a.dY + ci * a.dv * kPU;
+  if (tid < 3) mbar_init(&bars[tid], 1);
+  __syncthreads();
+  auto load = [&](int v0, int buf) {    // one thread
+    const uint32_t nv = (uint32_t)min(kVB, a.dv - v0);
+    float* f = F + buf * L::set;
+    uint64_t* bar = &bars[buf];
+    mbar_expect_tx(bar, nv * (2 * L::PS + 2 * kPU) * 4);
+    bulk_g2s(f, gS + (int64_t)v0 * L::PS, nv * L::PS * 4, bar);
+    bulk_g2s(f + L::ds, gDS + (int64_t)v0 * L::PS, nv * L::PS * 4, bar);
+    bulk_g2s(f + L::u, gU + (int64_t)v0 * kPU, nv * kPU * 4, bar);
+    bulk_g2s(f + L::dy, gY + (int64_t)v0 * kPU, nv * kPU * 4, bar);
+  };
+  // columns past dv of the last block count as zero
+  auto blank = [&](int v0, int buf) {
+    const int nv = a.dv - v0;
+    if (nv >= kVB) return;
+    float* f = F + buf * L::set;
+    for (int i = tid; i < (kVB - nv) * L::PS; i += kT) f[nv * L::PS + i] = f[L::ds + nv * L::PS + i] = 0.f;
+    for (int i = tid; i < (kVB - nv) * kPU; i += kT) f[L::u + nv * kPU + i] = f[L::dy + nv * kPU + i] = 0.f;
+  };
+  const int64_t os = (int64_t)a.Hv * a.dv;
+  const int tok = tid >> 3, vc = (tid & 7) * 4;      // this thread's values of dO and V
+  const E* dop = static_cast<const E*>(a.dout) + ((int64_t)b * a.T + t0 + tok) * os + (int64_t)h * a.dv + vc;
+  const E* vp = static_cast<const E*>(a.v) + b * a.vs[0] + (t0 + tok) * a.vs[1] + h * a.vs[2] + vc;
+  E xo[4], xv[4];
+  auto fetch = [&](int v0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool ok = tok < rows && v0 + vc + i < a.dv;
+      xo[i] = ok ? dop[v0 + i] : from_f<E>(0.f);
+      xv[i] = ok ? vp[v0 + i] : from_f<E>(0.f);
+    }
+  };
+  if (tid == 0) {
+    mbar_expect_tx(&bars[2], (uint32_t)(2 * L::tile) + kVec * 4);
+    bulk_g2s(smem, static_cast<const unsigned char*>(a.kq) + (((int64_t)b * a.Hk + hk) * a.NC + chunk) * (2 * L::tile),
+             (uint32_t)(2 * L::tile), &bars[2]);
+    bulk_g2s(eG, a.rec + ci * kRecord + 2 * kTri, kVec * 4, &bars[2]);
+    load(0, 0);
   }
-  for (int i = tid; i < kVec / 4; i += 256) cp16(eG + i * 4, a.rec + ci * kRecord + 2 * kTri + i * 4, true);
-  cp_commit();
+  blank(0, 0);
+  fetch(0);
 
-  float d1[2][NC4][4], dqa[2][NC4][4], d3[2][NC4][4], dp[2][2][4], da[2][2][4];
+  float d1[2][N][4], dqa[2][N][4], d3[2][N][4], dp[2][4], da[2][4];
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
 #pragma unroll
-    for (int n = 0; n < NC4; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) d1[m][n][i] = dqa[m][n][i] = d3[m][n][i] = 0.f;
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) dp[m][n][i] = da[m][n][i] = 0.f;
+    for (int n = 0; n < N; ++n) {
+      clear(d1[m][n]);
+      clear(dqa[m][n]);
+      clear(d3[m][n]);
+    }
+    clear(dp[m]);
+    clear(da[m]);
   }
   float ss = 0.f;     // <S0, dS>
-  float yv = 0.f;     // dY.V of token tid >> 2, columns tid & 3 mod 4
-  const int64_t os = (int64_t)a.Hv * a.dv;
-  const E* dop = static_cast<const E*>(a.dout) + ((int64_t)b * a.T + t0) * os + (int64_t)h * a.dv;
-  const E* vp = static_cast<const E*>(a.v) + b * a.vs[0] + t0 * a.vs[1] + h * a.vs[2];
-  const float* gS = a.Sn + ci * a.dv * DK;
-  const float* gDS = a.dS + ci * a.dv * DK;
-  const float* gU = a.U + ci * a.dv * kC;
-  const float* gY = a.dY + ci * a.dv * kC;
-
-  for (int v0 = 0; v0 < a.dv; v0 += kVB) {
-    const int nv = min(kVB, a.dv - v0);
+  float yv = 0.f;     // dY.V of this thread's token, its columns
+  bool there = true;
+  int blk = 0;
+  for (int v0 = 0; v0 < a.dv; v0 += kVB, ++blk) {
+    const int buf = blk & 1;
+    const float* f = F + buf * L::set;
+    *reinterpret_cast<float4*>(sDO + tok * L::PO + vc) =
+        make_float4(to_f<E>(xo[0]), to_f<E>(xo[1]), to_f<E>(xo[2]), to_f<E>(xo[3]));
+    const float v[4] = {to_f<E>(xv[0]), to_f<E>(xv[1]), to_f<E>(xv[2]), to_f<E>(xv[3])};
+    if (v0 + kVB < a.dv) {
+      if (tid == 0) load(v0 + kVB, buf ^ 1);
+      blank(v0 + kVB, buf ^ 1);
+      fetch(v0 + kVB);
+    }
+    there &= stage_wait(&bars[buf], (blk >> 1) & 1);
     __syncthreads();
-    for (int i = tid; i < kVB * DK / 4; i += 256) {
-      const int r = i / (DK / 4), c = (i - r * (DK / 4)) * 4;
-      const bool ok = r < nv;
-      const int64_t at = ok ? (int64_t)(v0 + r) * DK + c : 0;
-      cp16(sS0 + r * L::PS + c, gS + at, ok);
-      cp16(sDS + r * L::PS + c, gDS + at, ok);
-    }
-    for (int i = tid; i < kVB * kC / 4; i += 256) {
-      const int r = i / (kC / 4), c = (i - r * (kC / 4)) * 4;
-      const bool ok = r < nv;
-      const int64_t at = ok ? (int64_t)(v0 + r) * kC + c : 0;
-      cp16(sU + r * L::PY + c, gU + at, ok);
-      cp16(sDY + r * L::PY + c, gY + at, ok);
-    }
-    cp_commit();
-    for (int i = tid; i < kC * kVB; i += 256) {
-      const int r = i / kVB, c = i - r * kVB;
-      const bool ok = r < rows && c < nv;
-      sDO[r * L::PO + c] = ok ? to_f<E>(dop[r * os + v0 + c]) : 0.f;
-      sV[r * L::PO + c] = ok ? to_f<E>(vp[r * a.vs[1] + v0 + c]) : 0.f;
-    }
-    cp_wait<0>();
-    __syncthreads();
-    // <S0, dS> and dY.V in 32-bit arithmetic
-    for (int i = tid; i < kVB * DK; i += 256) {
-      const int r = i / DK, c = i - r * DK;
-      ss = fmaf(sS0[r * L::PS + c], sDS[r * L::PS + c], ss);
-    }
-    {
-      const int tok = tid >> 2;
 #pragma unroll
-      for (int c = 0; c < kVB / 4; ++c) {
-        const int v = c * 4 + (tid & 3);
-        yv = fmaf(sDY[v * L::PY + tok], sV[tok * L::PO + v], yv);
-      }
+    for (int i = 0; i < 4; ++i) yv = fmaf(f[L::dy + (vc + i) * kPU + tok], v[i], yv);
+    for (int i = tid; i < kVB * DK / 4; i += kT) {
+      const int at = (i / (DK / 4)) * L::PS + (i % (DK / 4)) * 4;
+      const float4 x = *reinterpret_cast<const float4*>(f + at), y = *reinterpret_cast<const float4*>(f + L::ds + at);
+      ss += (x.x * y.x + x.y * y.y) + (x.z * y.z + x.w * y.w);
     }
-#pragma unroll
-    for (int ks = 0; ks < kVB / 8; ++ks) {
-      const int vr = ks * 8 + 2 * t;
-      float oh[2][4], ol[2][4], yh[2][4], yl[2][4], uh[2][4], ul[2][4];
+    // each block's sums are started afresh and added in one rounding (the tensor unit cuts its sums)
+    float t1[2][N][4], t2[2][4];
+    auto zero = [&] {
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        const int i = wr * 32 + m * 16 + g;
-        const float2 p0 = pair(sDO + i * L::PO + vr), p1 = pair(sDO + (i + 8) * L::PO + vr);
-        const float ao[4] = {p0.x, p1.x, p0.y, p1.y};
-        if (X) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) oh[m][e] = ao[e];
-        } else {
-          split4(ao, oh[m], ol[m]);
-        }
-        const float* y = sDY + vr * L::PY + i;
-        const float ay[4] = {y[0], y[8], y[L::PY], y[L::PY + 8]};
-        split4(ay, yh[m], yl[m]);
-        const float* u = sU + vr * L::PY + i;
-        const float au[4] = {u[0], u[8], u[L::PY], u[L::PY + 8]};
-        split4(au, uh[m], ul[m]);
+        for (int n = 0; n < N; ++n) clear(t1[m][n]);
+        clear(t2[m]);
       }
+    };
+    auto add = [&](float (*x1)[N][4], float (*x2)[4]) {
 #pragma unroll
-      for (int n = 0; n < NC4; ++n) {
-        const int col = wc * (DK / 4) + n * 8 + g;
-        float h0, l0, h1, l1;
-        split(sS0[vr * L::PS + col], h0, l0);
-        split(sS0[(vr + 1) * L::PS + col], h1, l1);
+      for (int m = 0; m < 2; ++m) {
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          mma(d1[m][n], yl[m], h0, h1);
-          mma(dqa[m][n], oh[m], l0, l1);
-          mma(d1[m][n], yh[m], l0, l1);
-          if (!X) mma(dqa[m][n], ol[m], h0, h1);
-          mma(d1[m][n], yh[m], h0, h1);
-          mma(dqa[m][n], oh[m], h0, h1);
-        }
-        split(sDS[vr * L::PS + col], h0, l0);
-        split(sDS[(vr + 1) * L::PS + col], h1, l1);
+        for (int n = 0; n < N; ++n)
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          mma(d3[m][n], ul[m], h0, h1);
-          mma(d3[m][n], uh[m], l0, l1);
-          mma(d3[m][n], uh[m], h0, h1);
-        }
+          for (int i = 0; i < 4; ++i) x1[m][n][i] += t1[m][n][i];
+        if (x2)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x2[m][i] += t2[m][i];
       }
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const int col = wc * 16 + n * 8 + g;
-        float h0, l0, h1, l1;
-        split(sU[vr * L::PY + col], h0, l0);
-        split(sU[(vr + 1) * L::PY + col], h1, l1);
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          mma(dp[m][n], oh[m], l0, l1);
-          if (!X) mma(dp[m][n], ol[m], h0, h1);
-          mma(dp[m][n], oh[m], h0, h1);
-          mma(da[m][n], yl[m], h0, h1);
-          mma(da[m][n], yh[m], l0, l1);
-          mma(da[m][n], yh[m], h0, h1);
-        }
-      }
-    }
+    };
+    const float* s0 = f + wc * (DK / 8);
+    const float* u8 = f + L::u + wc * 8;
+    zero();
+    block_products<false, false, N, true>(t1, t2, f + L::dy + wr * 32, kPU, s0, L::PS, u8, kPU, g, t);
+    add(d1, da);
+    zero();
+    block_products<X, true, N, true>(t1, t2, sDO + wr * 32 * L::PO, L::PO, s0, L::PS, u8, kPU, g, t);
+    add(dqa, dp);
+    zero();
+    block_products<false, false, N, false>(t1, t2, f + L::u + wr * 32, kPU, s0 + L::ds, L::PS, u8, kPU, g, t);
+    add(d3, nullptr);
+    __syncthreads();
   }
-  __syncthreads();
+  there &= stage_wait(&bars[2], 0);
+  if (!there) yv = ss = d1[0][0][0] = dqa[0][0][0] = __int_as_float(0x7fffffff);
 
   // dot products over the key rows
-  float pk1[4], pkq[4], pk3[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) {   // row wr * 32 + (r >> 1) * 16 + (r & 1) * 8 + g
     const int i = wr * 32 + (r >> 1) * 16 + (r & 1) * 8 + g;
     float x1 = 0.f, xq = 0.f, x3 = 0.f;
 #pragma unroll
-    for (int n = 0; n < NC4; ++n) {
-      const int col = wc * (DK / 4) + n * 8 + 2 * t;
+    for (int n = 0; n < N; ++n) {
+      const int col = wc * (DK / 8) + n * 8 + 2 * t;
       const float2 kk = pair(K + i * L::PK + col), qq = pair(Q + i * L::PK + col);
       const int e = 2 * (r & 1);
       x1 += kk.x * d1[r >> 1][n][e] + kk.y * d1[r >> 1][n][e + 1];
@@ -538,55 +571,57 @@ __global__ void __launch_bounds__(256) backward_chunk_kernel(Args a) {
       xq += __shfl_xor_sync(0xffffffffu, xq, o);
       x3 += __shfl_xor_sync(0xffffffffu, x3, o);
     }
-    pk1[r] = x1; pkq[r] = xq; pk3[r] = x3;
     if (t == 0) {
-      parts[(6 + wc) * kC + i] = pk1[r];
-      parts[(10 + wc) * kC + i] = pkq[r];
-      parts[(14 + wc) * kC + i] = pk3[r];
+      parts[(10 + wc) * kC + i] = x1;
+      parts[(18 + wc) * kC + i] = xq;
+      parts[(26 + wc) * kC + i] = x3;
     }
   }
-  yv += __shfl_xor_sync(0xffffffffu, yv, 1);
-  yv += __shfl_xor_sync(0xffffffffu, yv, 2);
-  if ((tid & 3) == 0) parts[18 * kC + (tid >> 2)] = yv;
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) yv += __shfl_xor_sync(0xffffffffu, yv, o);
+  if ((tid & 7) == 0) parts[34 * kC + tok] = yv;
   ss = warp_sum(ss);
-  if (lane == 0) parts[20 * kC + warp] = ss;
+  if (lane == 0) parts[35 * kC + warp] = ss;
 
   // E, F and the sums of dP P + dA A, dA (A/beta)
   float* sE = F + L::e;
   float* sF = F + L::f;
   const float* Pm = a.rec + ci * kRecord + kTri;
   const float* Bm = a.Bm + ci * kTri;
-  float cs[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+  float cs[2] = {0.f, 0.f};
   float bsum[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int i = wr * 32 + (r >> 1) * 16 + (r & 1) * 8 + g;
+    const int j0 = wc * 8 + 2 * t;
     float rs = 0.f, bsr = 0.f;
+    float2 pm = make_float2(0.f, 0.f), bm = pm, ev = pm, fv = pm;
+    if (wc <= (i >> 3)) {
+      const int at = tri(i >> 3, wc) + (i & 7) * 8 + 2 * t;
+      pm = *reinterpret_cast<const float2*>(Pm + at);
+      bm = *reinterpret_cast<const float2*>(Bm + at);
+    }
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int j = wc * 16 + n * 8 + 2 * t + e;
-        float ev = 0.f, fv = 0.f;
-        if (j <= i) {
-          const float gam = expf((gHi[i] - gHi[j]) + (gLo[i] - gLo[j]));
-          const float dpv = dp[r >> 1][n][2 * (r & 1) + e];
-          const int at = tri(i >> 3, j >> 3) + (i & 7) * 8 + (j & 7);
-          float m = dpv * Pm[at];
-          ev = a.scale * gam * dpv;
-          if (j < i) {
-            const float dav = -da[r >> 1][n][2 * (r & 1) + e];
-            const float nb = dav * Bm[at];
-            bsr += nb;
-            m = fmaf(beta[i], nb, m);
-            fv = beta[i] * gam * dav;
-          }
-          rs += m;
-          cs[n][e] += m;
+    for (int e = 0; e < 2; ++e) {
+      const int j = j0 + e;
+      if (j <= i) {
+        const float gam = expf((gHi[i] - gHi[j]) + (gLo[i] - gLo[j]));
+        const float dpv = dp[r >> 1][2 * (r & 1) + e];
+        float m = dpv * (e ? pm.y : pm.x);
+        (e ? ev.y : ev.x) = a.scale * gam * dpv;
+        if (j < i) {
+          const float dav = -da[r >> 1][2 * (r & 1) + e];
+          const float nb = dav * (e ? bm.y : bm.x);
+          bsr += nb;
+          m = fmaf(beta[i], nb, m);
+          (e ? fv.y : fv.x) = beta[i] * gam * dav;
         }
-        sE[i * L::PE + j] = ev;
-        sF[i * L::PE + j] = fv;
+        rs += m;
+        cs[e] += m;
       }
+    }
+    *reinterpret_cast<float2*>(sE + i * L::PE + j0) = ev;
+    *reinterpret_cast<float2*>(sF + i * L::PE + j0) = fv;
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
       rs += __shfl_xor_sync(0xffffffffu, rs, o);
@@ -596,14 +631,12 @@ __global__ void __launch_bounds__(256) backward_chunk_kernel(Args a) {
     bsum[r] = bsr;
   }
 #pragma unroll
-  for (int n = 0; n < 2; ++n)
+  for (int e = 0; e < 2; ++e) {
+    float x = cs[e];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float x = cs[n][e];
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-      if (g == 0) parts[(4 + wr) * kC + wc * 16 + n * 8 + 2 * t + e] = x;
-    }
+    for (int o = 4; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    if (g == 0) parts[(8 + wr) * kC + wc * 8 + 2 * t + e] = x;
+  }
   __syncthreads();
 
   // gates: thread i < 64 has token i
@@ -611,15 +644,15 @@ __global__ void __launch_bounds__(256) backward_chunk_kernel(Args a) {
   if (tid < kC) {
     const int i = tid;
     float c1 = 0.f, cq = 0.f, c3 = 0.f, rs = 0.f;
-    for (int p = 0; p < 4; ++p) {
-      c1 += parts[(6 + p) * kC + i];
-      cq += parts[(10 + p) * kC + i];
-      c3 += parts[(14 + p) * kC + i];
+    for (int p = 0; p < 8; ++p) {
       rs += parts[p * kC + i];
+      c1 += parts[(10 + p) * kC + i];
+      cq += parts[(18 + p) * kC + i];
+      c3 += parts[(26 + p) * kC + i];
     }
-    const float cc = parts[4 * kC + i] + parts[5 * kC + i];
+    const float cc = parts[8 * kC + i] + parts[9 * kC + i];
     const float L3 = eD[i] * c3;
-    dbe = parts[18 * kC + i] - eG[i] * c1;
+    dbe = parts[34 * kC + i] - eG[i] * c1;
     dG = (rs - cc) - beta[i] * eG[i] * c1 + a.scale * eG[i] * cq - L3;
     tailC = L3;
   }
@@ -629,22 +662,21 @@ __global__ void __launch_bounds__(256) backward_chunk_kernel(Args a) {
     for (int r = 0; r < 4; ++r) parts[wc * kC + wr * 32 + (r >> 1) * 16 + (r & 1) * 8 + g] = bsum[r];
   }
   if (tid < kC) {
-    parts[4 * kC + tid] = dG;
-    parts[5 * kC + tid] = tailC;
+    parts[8 * kC + tid] = dG;
+    parts[9 * kC + tid] = tailC;
   }
   __syncthreads();
   if (tid < kC) {
-    const int i = tid;
-    dbe += (parts[i] + parts[kC + i]) + (parts[2 * kC + i] + parts[3 * kC + i]);
-    if (i < rows) a.dbeta[((int64_t)b * a.T + t0 + i) * a.Hv + h] = dbe;
+    for (int p = 0; p < 8; ++p) dbe += parts[p * kC + tid];
+    if (tid < rows) a.dbeta[((int64_t)b * a.T + t0 + tid) * a.Hv + h] = dbe;
   }
   if (warp == 2) {   // dg: sums of dG from the end; the chunk's last G takes the tail terms
-    const float* sdG = parts + 4 * kC;
-    const float* sTail = parts + 5 * kC;
-    float x0 = sdG[2 * lane], x1 = sdG[2 * lane + 1];
+    const float* sdG = parts + 8 * kC;
+    const float* sTail = parts + 9 * kC;
+    const float x0 = sdG[2 * lane], x1 = sdG[2 * lane + 1];
     float tail = warp_sum(sTail[2 * lane] + sTail[2 * lane + 1]);
     float in = 0.f;
-    for (int p = 0; p < 8; ++p) in += parts[20 * kC + p];
+    for (int p = 0; p < kT / 32; ++p) in += parts[35 * kC + p];
     tail += eG[kC - 1] * in;
     float s = x0 + x1;
 #pragma unroll
@@ -661,60 +693,57 @@ __global__ void __launch_bounds__(256) backward_chunk_kernel(Args a) {
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int n = 0; n < NC4; ++n)
+    for (int n = 0; n < N; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int tok = wr * 32 + m * 16 + g + 8 * (i >> 1);
-        dqa[m][n][i] *= a.scale * eG[tok];
-        d1[m][n][i] = fmaf(-beta[tok] * eG[tok], d1[m][n][i], eD[tok] * d3[m][n][i]);
+        const int r = wr * 32 + m * 16 + g + 8 * (i >> 1);
+        dqa[m][n][i] *= a.scale * eG[r];
+        d1[m][n][i] = fmaf(-beta[r] * eG[r], d1[m][n][i], eD[r] * d3[m][n][i]);
       }
-#pragma unroll
+#pragma unroll 2
   for (int ks = 0; ks < 8; ++ks) {
-    float eh[2][4], el[2][4], th[2][4], tl[2][4], fh[2][4], fl[2][4];
     const int c0 = ks * 8 + 2 * t;
+    float2 kk[N], qq[N];
+    tiles_by_row<N>(kk, K + ks * 8 * L::PK + wc * (DK / 8), L::PK, lane);
+    tiles_by_row<N>(qq, Q + ks * 8 * L::PK + wc * (DK / 8), L::PK, lane);
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-      const int i = wr * 32 + m * 16 + g;
-      const float2 p0 = pair(sE + i * L::PE + c0), p1 = pair(sE + (i + 8) * L::PE + c0);
-      const float ae[4] = {p0.x, p1.x, p0.y, p1.y};
-      const float* et = sE + c0 * L::PE + i;
-      const float at[4] = {et[0], et[8], et[L::PE], et[L::PE + 8]};
-      const float2 f0 = pair(sF + i * L::PE + c0), f1 = pair(sF + (i + 8) * L::PE + c0);
-      const float* ft = sF + c0 * L::PE + i;
-      const float af[4] = {f0.x + ft[0], f1.x + ft[8], f0.y + ft[L::PE], f1.y + ft[L::PE + 8]};
-      if (SHORT) {
+      const int i0 = wr * 32 + m * 16, i = i0 + g;
+      float hi[4], lo[4];
+      auto prepare = [&](const float* x) {
+        if (SHORT) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          eh[m][e] = tf32(ae[e]);
-          th[m][e] = tf32(at[e]);
-          fh[m][e] = tf32(af[e]);
+          for (int e = 0; e < 4; ++e) hi[e] = tf32(x[e]);
+        } else {
+          split4(x, hi, lo);
         }
-      } else {
-        split4(ae, eh[m], el[m]);
-        split4(at, th[m], tl[m]);
-        split4(af, fh[m], fl[m]);
+      };
+      auto product = [&](float (*c)[4], const float2* y) {
+        if (SHORT) {
+#pragma unroll
+          for (int n = 0; n < N; ++n) mma(c[n], hi, y[n].x, y[n].y);
+        } else {
+          mma_split<X, N>(c, hi, lo, y);
+        }
+      };
+      if (ks * 8 <= i0 + 15) {           // E is lower triangular
+        const float2 p0 = pair(sE + i * L::PE + c0), p1 = pair(sE + (i + 8) * L::PE + c0);
+        const float x[4] = {p0.x, p1.x, p0.y, p1.y};
+        prepare(x);
+        product(dqa[m], kk);
       }
-    }
-    float2 kk[NC4], qq[NC4];
-#pragma unroll
-    for (int n = 0; n < NC4; ++n) {
-      const int at = c0 * L::PK + wc * (DK / 4) + n * 8 + g;
-      kk[n] = make_float2(to_f<E>(K[at]), to_f<E>(K[at + L::PK]));
-      qq[n] = make_float2(to_f<E>(Q[at]), to_f<E>(Q[at + L::PK]));
-    }
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      if (SHORT) {
-#pragma unroll
-        for (int n = 0; n < NC4; ++n) mma(dqa[m][n], eh[m], kk[n].x, kk[n].y);
-#pragma unroll
-        for (int n = 0; n < NC4; ++n) mma(d1[m][n], th[m], qq[n].x, qq[n].y);
-#pragma unroll
-        for (int n = 0; n < NC4; ++n) mma(d1[m][n], fh[m], kk[n].x, kk[n].y);
-      } else {
-        mma_split<X, NC4>(dqa[m], eh[m], el[m], kk);
-        mma_split<X, NC4>(d1[m], th[m], tl[m], qq);
-        mma_split<X, NC4>(d1[m], fh[m], fl[m], kk);
+      if (ks * 8 + 7 >= i0) {
+        const float* et = sE + c0 * L::PE + i;
+        const float x[4] = {et[0], et[8], et[L::PE], et[L::PE + 8]};
+        prepare(x);
+        product(d1[m], qq);
+      }
+      {
+        const float2 f0 = pair(sF + i * L::PE + c0), f1 = pair(sF + (i + 8) * L::PE + c0);
+        const float* ft = sF + c0 * L::PE + i;
+        const float x[4] = {f0.x + ft[0], f1.x + ft[8], f0.y + ft[L::PE], f1.y + ft[L::PE + 8]};
+        prepare(x);
+        product(d1[m], kk);
       }
     }
   }
@@ -725,12 +754,12 @@ __global__ void __launch_bounds__(256) backward_chunk_kernel(Args a) {
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int n = 0; n < NC4; ++n)
+    for (int n = 0; n < N; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int tok = wr * 32 + m * 16 + g + 8 * (i >> 1), col = wc * (DK / 4) + n * 8 + 2 * t + (i & 1);
-        if (tok >= rows || col >= a.dk) continue;
-        const int64_t at = ob + tok * ots + col;
+        const int r = wr * 32 + m * 16 + g + 8 * (i >> 1), col = wc * (DK / 8) + n * 8 + 2 * t + (i & 1);
+        if (r >= rows || col >= a.dk) continue;
+        const int64_t at = ob + r * ots + col;
         if (shared) {
           a.dq32[at] = dqa[m][n][i];
           a.dk32[at] = d1[m][n][i];
@@ -768,7 +797,7 @@ static int launch_chunks_typed(const Args& a, cudaStream_t st) {
   static std::atomic<uint64_t> seen;
   int rc = allow_smem(backward_chunk_kernel<E, DK>, bytes, seen);
   if (rc != BSX_OK) return rc;
-  backward_chunk_kernel<E, DK><<<(unsigned)((int64_t)a.B * a.Hv * a.NC), 256, bytes, st>>>(a);
+  backward_chunk_kernel<E, DK><<<(unsigned)((int64_t)a.B * a.Hv * a.NC), kChunkThreads, bytes, st>>>(a);
   BSX_LAUNCH_CHECK("plastic backward_chunk_kernel");
   if (a.Hk != a.Hv) {
     const int64_t n = (int64_t)a.B * a.T * a.Hk * a.dk;

@@ -3,8 +3,8 @@
 //
 // The K and Q tiles are also written back in the layout they have in shared memory, once per key head.
 // K K^T and Q K^T are 64x64xdk products (only the tiles on and below the diagonal); T = (I + A)^{-1} is built by
-// substitution: the four 16x16 diagonal blocks by columns (one lane each), then
-// T_ij = -T_ii sum_l A_il T_lj by block distance, in 32-bit arithmetic.  (A power series would need fewer steps but
+// substitution: the four 16x16 diagonal blocks by columns (one lane each), then by block distance
+// T_ij = -sum_l (T_ii A_il) T_lj, warp i having block row i, on split operands.  (A power series would need fewer steps but
 // loses all digits when the keys of a chunk are alike.)  The sums of g are taken in 64 bits and kept as two floats, so
 // that a strong decay (g is cut at -128, where e^g is 0 in 32 bits) leaves the differences behind it exact.
 #include "plastic.cuh"
@@ -14,10 +14,11 @@ namespace plastic {
 
 template <typename E, int DK>
 struct PrepLayout {
-  static constexpr int PK = sizeof(E) == 2 ? DK + 8 : DK + 8;  // pair loads of 8 rows hit distinct banks
+  static constexpr int PK = DK + 8;  // pair loads of 8 rows hit distinct banks
   static constexpr size_t tile = (size_t)kC * PK * sizeof(E);
-  static constexpr int PA = kC + 1;
-  static constexpr size_t bytes = 2 * tile + sizeof(float) * (2 * kC * PA + 3 * 256 + 4 * kC) + 16;
+  static constexpr int PA = kC + 4;  // as right operand rows 2t, 2t + 1 hit distinct banks
+  static_assert(2 * tile >= sizeof(float) * kC * PA, "T takes the place of the K and Q tiles");
+  static constexpr size_t bytes = 2 * tile + sizeof(float) * (kC * PA + 3 * kC);
 };
 
 template <typename E, int DK, bool BACK>
@@ -27,9 +28,8 @@ __global__ void __launch_bounds__(128) prepare_kernel(Args a) {
   E* sk = reinterpret_cast<E*>(smem);
   E* sq = reinterpret_cast<E*>(smem + L::tile);
   float* sA = reinterpret_cast<float*>(smem + 2 * L::tile);
-  float* sT = sA + kC * L::PA;
-  float* sW = sT + kC * L::PA;      // 3 x 16 x 16
-  float* sHi = sW + 3 * 256;
+  float* sT = reinterpret_cast<float*>(smem);      // once K and Q are not needed any more
+  float* sHi = sA + kC * L::PA;
   float* sLo = sHi + kC;
   float* sBeta = sLo + kC;
 
@@ -164,25 +164,54 @@ __global__ void __launch_bounds__(128) prepare_kernel(Args a) {
       sT[(16 * warp + i) * L::PA + 16 * warp + lane] = v;
     }
   }
-  __syncthreads();
-  for (int d = 1; d < 4; ++d) {
-    const int n = (4 - d) * 256;
-    for (int e = tid; e < n; e += 128) {
-      const int blk = e >> 8, r = (e >> 4) & 15, c = e & 15, j = blk, i = blk + d;
-      float v = 0.f;
-      for (int l = j * 16; l < i * 16; ++l) v = fmaf(sA[(i * 16 + r) * L::PA + l], sT[l * L::PA + j * 16 + c], v);
-      sW[e] = v;
-    }
-    __syncthreads();
-    for (int e = tid; e < n; e += 128) {
-      const int blk = e >> 8, r = (e >> 4) & 15, c = e & 15, j = blk, i = blk + d;
-      float v = 0.f;
+  __syncwarp();
+  // -T_ii A_il for l < i = warp, kept as left operands
+  float z[3][2][4];
 #pragma unroll
-      for (int l = 0; l < 16; ++l) v = fmaf(-sT[(i * 16 + r) * L::PA + i * 16 + l], sW[blk * 256 + l * 16 + c], v);
-      sT[(i * 16 + r) * L::PA + j * 16 + c] = v;
+  for (int l = 0; l < 3; ++l) {
+    if (l >= warp) break;
+    clear(z[l][0]);
+    clear(z[l][1]);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const float* p = sT + (16 * warp + g) * L::PA + 16 * warp + ks * 8 + 2 * t;
+      const float2 p0 = pair(p), p1 = pair(p + 8 * L::PA);
+      const float x[4] = {-p0.x, -p1.x, -p0.y, -p1.y};
+      float hi[4], lo[4];
+      split4(x, hi, lo);
+      const float* r = sA + (16 * warp + ks * 8 + 2 * t) * L::PA + 16 * l + g;
+      const float2 y[2] = {make_float2(r[0], r[L::PA]), make_float2(r[8], r[L::PA + 8])};
+      mma_split<false, 2>(z[l], hi, lo, y);
     }
-    __syncthreads();
   }
+  for (int d = 1; d < 4; ++d) {
+    __syncthreads();
+    const int j = warp - d;
+    if (j < 0) continue;
+    float c[2][4];
+    clear(c[0]);
+    clear(c[1]);
+#pragma unroll
+    for (int l = 0; l < 3; ++l) {
+      if (l < j || l >= warp) continue;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        float x[4], hi[4], lo[4];
+        as_left(z[l][ks], x);
+        split4(x, hi, lo);
+        const float* r = sT + (16 * l + ks * 8 + 2 * t) * L::PA + 16 * j + g;
+        const float2 y[2] = {make_float2(r[0], r[L::PA]), make_float2(r[8], r[L::PA + 8])};
+        mma_split<false, 2>(c, hi, lo, y);
+      }
+    }
+    float* o = sT + (16 * warp + g) * L::PA + 16 * j + 2 * t;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      *reinterpret_cast<float2*>(o + n * 8) = make_float2(c[n][0], c[n][1]);
+      *reinterpret_cast<float2*>(o + n * 8 + 8 * L::PA) = make_float2(c[n][2], c[n][3]);
+    }
+  }
+  __syncthreads();
   for (int n = warp; n < 8; n += 4)
     for (int k = 0; k <= n; ++k) {
       const float* x = sT + (n * 8 + g) * L::PA + k * 8 + 2 * t;

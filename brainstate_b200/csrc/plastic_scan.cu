@@ -162,13 +162,13 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(Args a, int groups, in
     const int64_t t0 = (int64_t)c * kC;
 
     if (SAVE) {  // the state before this chunk, transposed
-      float* Sn = a.Sn + ci * a.dv * DK;
+      float* Sn = a.Sn + ci * a.dv * (DK + 4);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf)
           if (d0 + 8 * hf < a.dv)
-            *reinterpret_cast<float2*>(Sn + (int64_t)(d0 + 8 * hf) * DK + kb + n * 8 + 2 * t) =
+            *reinterpret_cast<float2*>(Sn + (d0 + 8 * hf) * (DK + 4) + kb + n * 8 + 2 * t) =
                 make_float2(s[n][2 * hf], s[n][2 * hf + 1]);
     }
 #pragma unroll
@@ -224,9 +224,9 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(Args a, int groups, in
     for (int e = 0; e < 2; ++e) {
       const int tok = own[e] * 8 + 2 * t;
       if (SAVE) {
-        float* U = a.U + ci * a.dv * kC;
-        if (in0) *reinterpret_cast<float2*>(U + (int64_t)d0 * kC + tok) = make_float2(u[e][0], u[e][1]);
-        if (in1) *reinterpret_cast<float2*>(U + (int64_t)(d0 + 8) * kC + tok) = make_float2(u[e][2], u[e][3]);
+        float* U = a.U + ci * a.dv * kPU;
+        if (in0) *reinterpret_cast<float2*>(U + d0 * kPU + tok) = make_float2(u[e][0], u[e][1]);
+        if (in1) *reinterpret_cast<float2*>(U + (d0 + 8) * kPU + tok) = make_float2(u[e][2], u[e][3]);
       }
       if (OUT) gU[own[e] * 32 + lane] = make_float4(u[e][0], u[e][2], u[e][1], u[e][3]);
       const float2 ed = pair(eD + tok);
