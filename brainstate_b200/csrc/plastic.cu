@@ -145,6 +145,10 @@ extern "C" int bsx_delta_backward(const bsx_delta_t* d, const void* dout, const 
   if (a.NC > 0 && (!ws || !aligned16(ws) || ws_bytes < workspace(d, true)))
     return fail(BSX_ERR_WORKSPACE, "workspace missing, misaligned or too small");
   if (sm_count() <= 0) return fail(BSX_ERR_CUDA, "no CUDA device");
+  const uintptr_t four = 4 * (d->dtype == BSX_T_F32 ? 4 : 2) - 1;
+  a.four_do = a.dv % 4 == 0 && (reinterpret_cast<uintptr_t>(dout) & four) == 0;
+  a.four_v = a.dv % 4 == 0 && (reinterpret_cast<uintptr_t>(a.v) & four) == 0 && a.vs[0] % 4 == 0 && a.vs[1] % 4 == 0 &&
+             a.vs[2] % 4 == 0;
   a.dout = dout; a.dstate = dstate;
   a.dq = dq; a.dk_ = dk; a.dv_ = dv; a.dg = dg; a.dbeta = dbeta; a.dinitial = dinitial;
   place(a, d, static_cast<float*>(ws), true);

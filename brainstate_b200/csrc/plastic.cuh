@@ -53,6 +53,7 @@ struct Args {
   void *dq, *dk_, *dv_;
   float *dg, *dbeta, *dinitial;
   float *dq32, *dk32;     // per value head, when heads share keys
+  bool four_do, four_v;   // dO, V: four neighbouring elements can be loaded together
   bool vec_qk;            // rows of q and k start on 16-byte boundaries and are whole 16-byte stretches
 };
 

@@ -7,13 +7,16 @@
 //   dS <- e^{G_C} dS + Q^T (scale e^G dO) + K^T dR.
 // It leaves dS (before the update) and dY for every chunk.
 //
-// backward_chunk_kernel: everything else, all chunks at once, one block of 16 warps per (row, head, chunk).  Over blocks of 32
-// value columns (bulk copies, one block ahead) it sums D1 = dY S0^T, Dq = dO S0^T, D3 = U dS^T (64 x dk) and dP = dO U^T, dA = -dY U^T (64 x 64), then
+// backward_chunk_kernel: everything else, independent of the order of the chunks; each block of 16 warps takes every
+// gridDim-th (row, head, chunk) and copies the next one's data while it finishes one.  Over blocks of 32 value columns it
+// sums D1 = dY S0^T, Dq = dO S0^T, D3 = U dS^T (64 x dk) and dP = dO U^T, dA = -dY U^T (64 x 64), then
 //   dQ = scale e^G Dq + E K,                         E = scale Gamma dP (j <= i)
 //   dK = -beta e^G D1 + e^{G_C-G} D3 + E^T Q + (F + F^T) K,   F = beta Gamma dA (j < i)
 //   dbeta_i = dY_i.V_i - e^{G_i} K_i.D1_i + sum_j dA_ij (A/beta)_ij
 //   dG_i = -beta e^G K_i.D1_i + scale e^G Q_i.Dq_i - e^{G_C-G} K_i.D3_i + (row - column sums of dP P + dA A)_i,
 //   dG_C += sum_i e^{G_C-G_i} K_i.D3_i + e^{G_C} <S0, dS>,   dg = sums of dG from the chunk's end.
+#include <type_traits>
+
 #include "plastic.cuh"
 
 namespace bsx {
@@ -341,13 +344,66 @@ struct BackChunkLayout {
   static constexpr int PK = DK + 8, PS = DK + 4, PO = kVB + 8, PE = kC + 8;
   static constexpr size_t tile = (size_t)kC * PK * sizeof(E);
   // floats of one set of block buffers: S0, dS, U, dY
-  static constexpr int ds = kVB * PS, u = 2 * kVB * PS, dy = u + kVB * kPU, set = dy + kVB * kPU;
+  static constexpr int ds = kVB * PS, u = 2 * kVB * PS, dy = u + kVB * kPU, used = dy + kVB * kPU,
+                       set = used > 2 * kC * PE ? used : 2 * kC * PE;   // E and F have to fit as well
   // floats after the K and Q tiles
-  static constexpr int dof = 2 * set, vecs = dof + kC * PO, parts = vecs + kVec, end = parts + 36 * kC;
-  static constexpr int e = 0, f = kC * PE;       // reuse the block buffers
-  static_assert(2 * kC * PE <= 2 * set, "");
+  static constexpr int dof = 2 * set, pm = dof + kC * PO, vecs = pm + kTri, bm = vecs + kVec, parts = bm + kTri,
+                       end = parts + 36 * kC;
+  // E and F, then the finished gradients, take the set that the next chunk's first block does not
+  static constexpr int f = kC * PE;
   static constexpr size_t bytes = 2 * tile + (size_t)end * sizeof(float);
 };
+
+// Four neighbouring elements as they come from memory: taken apart only where they are used, so that a load a block ahead
+// is not waited for where it is issued.
+template <typename E> struct Four;
+template <> struct Four<float> {
+  float4 w;
+  __device__ __forceinline__ void load(const float* p) { w = *reinterpret_cast<const float4*>(p); }
+  __device__ __forceinline__ void gather(const float* p, int left) {
+    w.x = left > 0 ? p[0] : 0.f;
+    w.y = left > 1 ? p[1] : 0.f;
+    w.z = left > 2 ? p[2] : 0.f;
+    w.w = left > 3 ? p[3] : 0.f;
+  }
+  __device__ __forceinline__ float4 get() const { return w; }
+};
+template <typename H> struct FourHalves {
+  uint2 w;
+  __device__ __forceinline__ void load(const H* p) { w = *reinterpret_cast<const uint2*>(p); }
+  __device__ __forceinline__ void gather(const H* p, int left) {
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+    uint32_t v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < left ? q[i] : 0u;
+    w = make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
+  }
+  __device__ __forceinline__ float4 get() const {
+    const float2 a = unpack(w.x, (const H*)nullptr), b = unpack(w.y, (const H*)nullptr);
+    return make_float4(a.x, a.y, b.x, b.y);
+  }
+};
+template <> struct Four<__nv_bfloat16> : FourHalves<__nv_bfloat16> {};
+template <> struct Four<__half> : FourHalves<__half> {};
+
+// Rows of a finished (token, column) tile from shared memory, pitch `pitch`, to global memory.
+template <typename O>
+__device__ __forceinline__ void store_rows(O* dst, int64_t stride, const O* sm, int pitch, int rows, int cols, bool vec, int tid,
+                                           int nthr) {
+  constexpr int V = 16 / sizeof(O);
+  if (vec) {
+    const int per = cols / V;
+    for (int i = tid; i < rows * per; i += nthr) {
+      const int r = i / per, c = (i - r * per) * V;
+      *reinterpret_cast<int4*>(dst + r * stride + c) = *reinterpret_cast<const int4*>(sm + r * pitch + c);
+    }
+  } else {
+    for (int i = tid; i < rows * cols; i += nthr) {
+      const int r = i / cols, c = i - r * cols;
+      dst[r * stride + c] = sm[r * pitch + c];
+    }
+  }
+}
 
 // t[m][n] += a b over the four 8-column steps of a block: a (32 rows of this warp, two tiles) from a transposed (column,
 // row) array or, with ROWS, from a (row, column) one; b from two (column, outer) arrays, N tiles of the first and one of
@@ -411,6 +467,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) backward_chunk_kernel(Args a
   E* Q = reinterpret_cast<E*>(smem + L::tile);
   float* F = reinterpret_cast<float*>(smem + 2 * L::tile);
   float* sDO = F + L::dof;
+  const float* Pm = F + L::pm;
+  const float* Bm = F + L::bm;
   float* eG = F + L::vecs;
   float* eD = eG + kC;
   float* beta = eG + 2 * kC;
@@ -422,29 +480,34 @@ __global__ void __launch_bounds__(kChunkThreads, 1) backward_chunk_kernel(Args a
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int wr = warp & 1, wc = warp >> 1;     // rows 32 wr .. + 31; column eighth wc
-  const int chunk = blockIdx.x % a.NC;
-  const int bh = blockIdx.x / a.NC, b = bh / a.Hv, h = bh - b * a.Hv, hk = h / (a.Hv / a.Hk);
-  const int len = row_length(a, b);
-  const int64_t t0 = (int64_t)chunk * kC;
-  if (t0 >= len) return;
-  const int rows = (int)min((int64_t)kC, len - t0);
-  const int64_t ci = (int64_t)bh * a.NC + chunk;
+  const int64_t os = (int64_t)a.Hv * a.dv;
+  const int tok = tid >> 3, vc = (tid & 7) * 4;      // this thread's values of dO and V
+  const uint32_t items = (uint32_t)a.B * a.Hv * a.NC, NC = a.NC, Hv = a.Hv;
 
-  const float* gS = a.Sn + ci * a.dv * L::PS;
-  const float* gDS = a.dS + ci * a.dv * L::PS;
-  const float* gU = a.U + ci * a.dv * kPU;
-  const float* gY = a.dY + ci * a.dv * kPU;
-  if (tid < 3) mbar_init(&bars[tid], 1);
-  __syncthreads();
-  auto load = [&](int v0, int buf) {    // one thread
+  // the next item from `i` on that has tokens
+  auto valid = [&](uint32_t i) {
+    if (a.lengths)
+      while (i < items && (int)(i % NC) * kC >= row_length(a, (int)(i / NC / Hv))) i += gridDim.x;
+    return i;
+  };
+  auto load = [&](uint32_t ci, int v0, int buf) {    // one thread
     const uint32_t nv = (uint32_t)min(kVB, a.dv - v0);
     float* f = F + buf * L::set;
     uint64_t* bar = &bars[buf];
+    const int64_t row = (int64_t)ci * a.dv + v0;
     mbar_expect_tx(bar, nv * (2 * L::PS + 2 * kPU) * 4);
-    bulk_g2s(f, gS + (int64_t)v0 * L::PS, nv * L::PS * 4, bar);
-    bulk_g2s(f + L::ds, gDS + (int64_t)v0 * L::PS, nv * L::PS * 4, bar);
-    bulk_g2s(f + L::u, gU + (int64_t)v0 * kPU, nv * kPU * 4, bar);
-    bulk_g2s(f + L::dy, gY + (int64_t)v0 * kPU, nv * kPU * 4, bar);
+    bulk_g2s(f, a.Sn + row * L::PS, nv * L::PS * 4, bar);
+    bulk_g2s(f + L::ds, a.dS + row * L::PS, nv * L::PS * 4, bar);
+    bulk_g2s(f + L::u, a.U + row * kPU, nv * kPU * 4, bar);
+    bulk_g2s(f + L::dy, a.dY + row * kPU, nv * kPU * 4, bar);
+  };
+  auto load_chunk = [&](uint32_t ci) {    // one thread: K, Q, P, the vectors, A / beta
+    const uint32_t bh = ci / NC, b = bh / Hv, hk = (bh - b * Hv) / (Hv / a.Hk);
+    mbar_expect_tx(&bars[2], (uint32_t)(2 * L::tile) + (2 * kTri + kVec) * 4);
+    bulk_g2s(smem, static_cast<const unsigned char*>(a.kq) + (((int64_t)b * a.Hk + hk) * NC + ci % NC) * (2 * L::tile),
+             (uint32_t)(2 * L::tile), &bars[2]);
+    bulk_g2s(F + L::pm, a.rec + (int64_t)ci * kRecord + kTri, (kTri + kVec) * 4, &bars[2]);
+    bulk_g2s(F + L::bm, a.Bm + (int64_t)ci * kTri, kTri * 4, &bars[2]);
   };
   // columns past dv of the last block count as zero
   auto blank = [&](int v0, int buf) {
@@ -454,28 +517,36 @@ __global__ void __launch_bounds__(kChunkThreads, 1) backward_chunk_kernel(Args a
     for (int i = tid; i < (kVB - nv) * L::PS; i += kT) f[nv * L::PS + i] = f[L::ds + nv * L::PS + i] = 0.f;
     for (int i = tid; i < (kVB - nv) * kPU; i += kT) f[L::u + nv * kPU + i] = f[L::dy + nv * kPU + i] = 0.f;
   };
-  const int64_t os = (int64_t)a.Hv * a.dv;
-  const int tok = tid >> 3, vc = (tid & 7) * 4;      // this thread's values of dO and V
-  const E* dop = static_cast<const E*>(a.dout) + ((int64_t)b * a.T + t0 + tok) * os + (int64_t)h * a.dv + vc;
-  const E* vp = static_cast<const E*>(a.v) + b * a.vs[0] + (t0 + tok) * a.vs[1] + h * a.vs[2] + vc;
-  E xo[4], xv[4];
-  auto fetch = [&](int v0) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bool ok = tok < rows && v0 + vc + i < a.dv;
-      xo[i] = ok ? dop[v0 + i] : from_f<E>(0.f);
-      xv[i] = ok ? vp[v0 + i] : from_f<E>(0.f);
-    }
+  Four<E> xo, xv;
+  const E *po = nullptr, *pv = nullptr;     // this thread's dO and V of an item, at column vc; NULL past the sequence's end
+  auto locate = [&](uint32_t ci) {
+    const uint32_t bh = ci / NC, b = bh / Hv, h = bh - b * Hv;
+    const int64_t tk = (int64_t)(ci - bh * NC) * kC + tok;
+    po = tk < row_length(a, b) ? static_cast<const E*>(a.dout) + ((int64_t)b * a.T + tk) * os + (int64_t)h * a.dv + vc : nullptr;
+    pv = static_cast<const E*>(a.v) + b * a.vs[0] + tk * a.vs[1] + h * a.vs[2] + vc;
   };
-  if (tid == 0) {
-    mbar_expect_tx(&bars[2], (uint32_t)(2 * L::tile) + kVec * 4);
-    bulk_g2s(smem, static_cast<const unsigned char*>(a.kq) + (((int64_t)b * a.Hk + hk) * a.NC + chunk) * (2 * L::tile),
-             (uint32_t)(2 * L::tile), &bars[2]);
-    bulk_g2s(eG, a.rec + ci * kRecord + 2 * kTri, kVec * 4, &bars[2]);
-    load(0, 0);
+  auto fetch = [&](int v0) {
+    const int left = po ? a.dv - v0 - vc : 0;
+    if (left > 0 && a.four_do) xo.load(po + v0);       // dv is a multiple of four
+    else xo.gather(po + v0, left);
+    if (left > 0 && a.four_v) xv.load(pv + v0);
+    else xv.gather(pv + v0, left);
+  };
+
+  if (tid < 3) mbar_init(&bars[tid], 1);
+  __syncthreads();
+  uint32_t item = valid(blockIdx.x);
+  if (item < items) {
+    if (tid == 0) {
+      load(item, 0, 0);
+      load_chunk(item);
+    }
+    blank(0, 0);
+    locate(item);
+    fetch(0);
   }
-  blank(0, 0);
-  fetch(0);
+  uint32_t blk = 0;       // blocks taken so far: sets alternate across chunks
+  for (uint32_t nth = 0; item < items; ++nth) {
 
   float d1[2][N][4], dqa[2][N][4], d3[2][N][4], dp[2][4], da[2][4];
 #pragma unroll
@@ -492,15 +563,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) backward_chunk_kernel(Args a
   float ss = 0.f;     // <S0, dS>
   float yv = 0.f;     // dY.V of this thread's token, its columns
   bool there = true;
-  int blk = 0;
   for (int v0 = 0; v0 < a.dv; v0 += kVB, ++blk) {
     const int buf = blk & 1;
     const float* f = F + buf * L::set;
-    *reinterpret_cast<float4*>(sDO + tok * L::PO + vc) =
-        make_float4(to_f<E>(xo[0]), to_f<E>(xo[1]), to_f<E>(xo[2]), to_f<E>(xo[3]));
-    const float v[4] = {to_f<E>(xv[0]), to_f<E>(xv[1]), to_f<E>(xv[2]), to_f<E>(xv[3])};
+    *reinterpret_cast<float4*>(sDO + tok * L::PO + vc) = xo.get();
+    const float4 v4 = xv.get();
+    const float v[4] = {v4.x, v4.y, v4.z, v4.w};
     if (v0 + kVB < a.dv) {
-      if (tid == 0) load(v0 + kVB, buf ^ 1);
+      if (tid == 0) load(item, v0 + kVB, buf ^ 1);
       blank(v0 + kVB, buf ^ 1);
       fetch(v0 + kVB);
     }
@@ -548,7 +618,20 @@ __global__ void __launch_bounds__(kChunkThreads, 1) backward_chunk_kernel(Args a
     add(d3, nullptr);
     __syncthreads();
   }
-  there &= stage_wait(&bars[2], 0);
+  const uint32_t next = valid(item + gridDim.x);
+  const uint32_t bh = item / NC, b = bh / Hv, h = bh - b * Hv, hk = h / (Hv / a.Hk);
+  const int64_t t0 = (int64_t)(item - bh * NC) * kC;
+  const int rows = (int)min((int64_t)kC, row_length(a, b) - t0);
+  // the next chunk's first block goes to one set, E, F and the gradients to the other
+  float* sE = F + ((blk & 1) ^ 1) * L::set;
+  float* sF = sE + L::f;
+  if (next < items) {
+    if (tid == 0) load(next, 0, blk & 1);
+    blank(0, blk & 1);
+    locate(next);
+    fetch(0);
+  }
+  there &= stage_wait(&bars[2], nth & 1);
   if (!there) yv = ss = d1[0][0][0] = dqa[0][0][0] = __int_as_float(0x7fffffff);
 
   // dot products over the key rows
@@ -584,10 +667,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) backward_chunk_kernel(Args a
   if (lane == 0) parts[35 * kC + warp] = ss;
 
   // E, F and the sums of dP P + dA A, dA (A/beta)
-  float* sE = F + L::e;
-  float* sF = F + L::f;
-  const float* Pm = a.rec + ci * kRecord + kTri;
-  const float* Bm = a.Bm + ci * kTri;
   float cs[2] = {0.f, 0.f};
   float bsum[4];
 #pragma unroll
@@ -747,27 +826,38 @@ __global__ void __launch_bounds__(kChunkThreads, 1) backward_chunk_kernel(Args a
       }
     }
   }
-  const bool shared = a.Hk != a.Hv;
-  const int heads = shared ? a.Hv : a.Hk, ho = shared ? h : hk;
-  const int64_t ob = (((int64_t)b * a.T + t0) * heads + ho) * a.dk;
-  const int64_t ots = (int64_t)heads * a.dk;
+  __syncthreads();      // K, Q, E and F are free
+  if (tid == 0 && next < items) load_chunk(next);
+  auto finish = [&](auto* dq, auto* dk, int heads, int ho) {
+    using O = typename std::remove_pointer<decltype(dq)>::type;
+    O* sm = reinterpret_cast<O*>(sE);
+    const int64_t at = (((int64_t)b * a.T + t0) * heads + ho) * a.dk, stride = (int64_t)heads * a.dk;
+    const bool vec = a.dk % (16 / (int)sizeof(O)) == 0 && (reinterpret_cast<uintptr_t>(dq) & 15) == 0 &&
+                     (reinterpret_cast<uintptr_t>(dk) & 15) == 0;
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+    for (int which = 0; which < 2; ++which) {
+      if (which) __syncthreads();
 #pragma unroll
-    for (int n = 0; n < N; ++n)
+      for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = wr * 32 + m * 16 + g + 8 * (i >> 1), col = wc * (DK / 8) + n * 8 + 2 * t + (i & 1);
-        if (r >= rows || col >= a.dk) continue;
-        const int64_t at = ob + r * ots + col;
-        if (shared) {
-          a.dq32[at] = dqa[m][n][i];
-          a.dk32[at] = d1[m][n][i];
-        } else {
-          static_cast<E*>(a.dq)[at] = from_f<E>(dqa[m][n][i]);
-          static_cast<E*>(a.dk_)[at] = from_f<E>(d1[m][n][i]);
-        }
-      }
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            const float* c = which ? d1[m][n] : dqa[m][n];
+            O* o = sm + (wr * 32 + m * 16 + g + 8 * hf) * L::PK + wc * (DK / 8) + n * 8 + 2 * t;
+            o[0] = from_f<O>(c[2 * hf]);
+            o[1] = from_f<O>(c[2 * hf + 1]);
+          }
+      __syncthreads();
+      store_rows<O>((which ? dk : dq) + at, stride, sm, L::PK, rows, a.dk, vec, tid, kT);
+    }
+  };
+  if (a.Hk != a.Hv) finish(a.dq32, a.dk32, a.Hv, h);
+  else finish(static_cast<E*>(a.dq), static_cast<E*>(a.dk_), a.Hk, hk);
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // bulk copies will follow these writes
+  __syncthreads();      // the set is free
+  item = next;
+  }
 }
 
 // Gradients of keys and queries that several value heads share: 32-bit sums in head order.
@@ -797,7 +887,9 @@ static int launch_chunks_typed(const Args& a, cudaStream_t st) {
   static std::atomic<uint64_t> seen;
   int rc = allow_smem(backward_chunk_kernel<E, DK>, bytes, seen);
   if (rc != BSX_OK) return rc;
-  backward_chunk_kernel<E, DK><<<(unsigned)((int64_t)a.B * a.Hv * a.NC), kChunkThreads, bytes, st>>>(a);
+  const int64_t items = (int64_t)a.B * a.Hv * a.NC;
+  const int sms = sm_count();
+  backward_chunk_kernel<E, DK><<<(unsigned)(items < sms ? items : sms), kChunkThreads, bytes, st>>>(a);
   BSX_LAUNCH_CHECK("plastic backward_chunk_kernel");
   if (a.Hk != a.Hv) {
     const int64_t n = (int64_t)a.B * a.T * a.Hk * a.dk;
