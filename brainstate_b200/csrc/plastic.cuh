@@ -47,6 +47,7 @@ struct Args {
   void* o;
   float* state;
   // backward
+  uint32_t* taken;      // chunks that blocks took beyond their first; cleared by the preparing kernel
   const void* dout;
   const float* dstate;
   float *dS, *dY;

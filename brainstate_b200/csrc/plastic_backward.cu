@@ -7,8 +7,8 @@
 //   dS <- e^{G_C} dS + Q^T (scale e^G dO) + K^T dR.
 // It leaves dS (before the update) and dY for every chunk.
 //
-// backward_chunk_kernel: everything else, independent of the order of the chunks; each block of 16 warps takes every
-// gridDim-th (row, head, chunk) and copies the next one's data while it finishes one.  Over blocks of 32 value columns it
+// backward_chunk_kernel: everything else, independent of the order of the chunks; each block of 16 warps takes one (row, head,
+// chunk) after the other and copies the next one's data while it finishes one.  Over blocks of 32 value columns it
 // sums D1 = dY S0^T, Dq = dO S0^T, D3 = U dS^T (64 x dk) and dP = dO U^T, dA = -dY U^T (64 x 64), then
 //   dQ = scale e^G Dq + E K,                         E = scale Gamma dP (j <= i)
 //   dK = -beta e^G D1 + e^{G_C-G} D3 + E^T Q + (F + F^T) K,   F = beta Gamma dA (j < i)
@@ -411,13 +411,20 @@ __device__ __forceinline__ void store_rows(O* dst, int64_t stride, const O* sm, 
 template <bool AEXACT, bool ROWS, int N, bool SECOND>
 __device__ __forceinline__ void block_products(float (*t1)[N][4], float (*t2)[4], const float* a, int pa, const float* b1, int p1,
                                                const float* b2, int p2, int g, int t) {
-#pragma unroll
+#pragma unroll 1   // unrolled, the accumulators (112 of 128 registers) do not stay in registers: 463 -> 521 us
   for (int ks = 0; ks < kVB / 8; ++ks) {
     const int v = ks * 8 + 2 * t;
-    float hi[2][4], lo[2][4];
+    constexpr int M = N + (SECOND ? 1 : 0);
+    float2 h[M], l[M];
+#pragma unroll
+    for (int n = 0; n < M; ++n) {
+      const float* p = n < N ? b1 + v * p1 + n * 8 + g : b2 + v * p2 + g;
+      split(p[0], h[n].x, l[n].x);
+      split(p[n < N ? p1 : p2], h[n].y, l[n].y);
+    }
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-      float x[4];
+      float x[4], hi[4], lo[4];
       if (ROWS) {
         const float2 p0 = pair(a + (m * 16 + g) * pa + v), q0 = pair(a + (m * 16 + g + 8) * pa + v);
         x[0] = p0.x; x[1] = q0.x; x[2] = p0.y; x[3] = q0.y;
@@ -427,29 +434,18 @@ __device__ __forceinline__ void block_products(float (*t1)[N][4], float (*t2)[4]
       }
       if (AEXACT) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) hi[m][i] = x[i];
+        for (int i = 0; i < 4; ++i) hi[i] = x[i];
       } else {
-        split4(x, hi[m], lo[m]);
+        split4(x, hi, lo);
       }
-    }
-    float2 h[N + 1], l[N + 1];
+      auto at = [&](int n) { return n < N ? t1[m][n < N ? n : 0] : t2[m]; };
+      if (!AEXACT)
 #pragma unroll
-    for (int n = 0; n < N + (SECOND ? 1 : 0); ++n) {
-      const float* p = n < N ? b1 + v * p1 + n * 8 + g : b2 + v * p2 + g;
-      split(p[0], h[n].x, l[n].x);
-      split(p[n < N ? p1 : p2], h[n].y, l[n].y);
-    }
+        for (int n = 0; n < M; ++n) mma(at(n), lo, h[n].x, h[n].y);
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
+      for (int n = 0; n < M; ++n) mma(at(n), hi, l[n].x, l[n].y);
 #pragma unroll
-      for (int n = 0; n < N + (SECOND ? 1 : 0); ++n) {
-        float* c = n < N ? t1[m][n < N ? n : 0] : t2[m];
-        if (!AEXACT) mma(c, lo[m], h[n].x, h[n].y);
-      }
-#pragma unroll
-      for (int n = 0; n < N + (SECOND ? 1 : 0); ++n) mma(n < N ? t1[m][n < N ? n : 0] : t2[m], hi[m], l[n].x, l[n].y);
-#pragma unroll
-      for (int n = 0; n < N + (SECOND ? 1 : 0); ++n) mma(n < N ? t1[m][n < N ? n : 0] : t2[m], hi[m], h[n].x, h[n].y);
+      for (int n = 0; n < M; ++n) mma(at(n), hi, h[n].x, h[n].y);
     }
   }
 }
@@ -463,6 +459,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) backward_chunk_kernel(Args a
   constexpr int kT = kChunkThreads;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ __align__(8) uint64_t bars[3];
+  __shared__ uint32_t next_item;
   E* K = reinterpret_cast<E*>(smem);
   E* Q = reinterpret_cast<E*>(smem + L::tile);
   float* F = reinterpret_cast<float*>(smem + 2 * L::tile);
@@ -484,10 +481,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) backward_chunk_kernel(Args a
   const int tok = tid >> 3, vc = (tid & 7) * 4;      // this thread's values of dO and V
   const uint32_t items = (uint32_t)a.B * a.Hv * a.NC, NC = a.NC, Hv = a.Hv;
 
-  // the next item from `i` on that has tokens
-  auto valid = [&](uint32_t i) {
+  // Where rows differ in length, items are taken as blocks become free; the first is the block's own number.
+  auto ask = [&](uint32_t i) { return a.lengths ? gridDim.x + atomicAdd(a.taken, 1u) : i + gridDim.x; };
+  auto valid = [&](uint32_t i) {    // the first from i on that has tokens
     if (a.lengths)
-      while (i < items && (int)(i % NC) * kC >= row_length(a, (int)(i / NC / Hv))) i += gridDim.x;
+      while (i < items && (int)(i % NC) * kC >= row_length(a, (int)(i / NC / Hv))) i = ask(i);
     return i;
   };
   auto load = [&](uint32_t ci, int v0, int buf) {    // one thread
@@ -535,7 +533,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) backward_chunk_kernel(Args a
 
   if (tid < 3) mbar_init(&bars[tid], 1);
   __syncthreads();
-  uint32_t item = valid(blockIdx.x);
+  if (tid == 0) next_item = valid(blockIdx.x);
+  __syncthreads();
+  uint32_t item = next_item;
   if (item < items) {
     if (tid == 0) {
       load(item, 0, 0);
@@ -547,6 +547,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) backward_chunk_kernel(Args a
   }
   uint32_t blk = 0;       // blocks taken so far: sets alternate across chunks
   for (uint32_t nth = 0; item < items; ++nth) {
+  uint32_t asked = 0;    // looked at after the blocks: the answer takes its time
+  if (tid == 0) asked = ask(item);
 
   float d1[2][N][4], dqa[2][N][4], d3[2][N][4], dp[2][4], da[2][4];
 #pragma unroll
@@ -618,7 +620,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) backward_chunk_kernel(Args a
     add(d3, nullptr);
     __syncthreads();
   }
-  const uint32_t next = valid(item + gridDim.x);
+  if (tid == 0) next_item = valid(asked);
+  __syncthreads();
+  const uint32_t next = next_item;
   const uint32_t bh = item / NC, b = bh / Hv, h = bh - b * Hv, hk = h / (Hv / a.Hk);
   const int64_t t0 = (int64_t)(item - bh * NC) * kC;
   const int rows = (int)min((int64_t)kC, row_length(a, b) - t0);

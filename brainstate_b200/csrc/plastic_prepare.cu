@@ -33,6 +33,7 @@ __global__ void __launch_bounds__(128) prepare_kernel(Args a) {
   float* sLo = sHi + kC;
   float* sBeta = sLo + kC;
 
+  if (BACK && blockIdx.x == 0 && threadIdx.x == 0) *a.taken = 0u;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int chunk = blockIdx.x % a.NC;
   const int bh = blockIdx.x / a.NC, b = bh / a.Hv, h = bh - b * a.Hv, hk = h / (a.Hv / a.Hk);

@@ -53,8 +53,7 @@ def _describe(q, k, v, g, beta, initial, lengths, scale) -> bytes:
 def _forward(q, k, v, g, beta, initial, lengths, scale):
     B, T, _, dk = q.shape
     Hv, dv = v.shape[2:]
-    # tokens past a row's length are not written by the kernels
-    o = v.new_empty((B, T, Hv, dv)) if lengths is None else v.new_zeros((B, T, Hv, dv))
+    o = v.new_empty((B, T, Hv, dv))
     state = g.new_empty((B, Hv, dk, dv))
     d = _describe(q, k, v, g, beta, initial, lengths, scale)
     if T <= RECURRENT_TOKENS:
@@ -81,9 +80,8 @@ class _DeltaRule(torch.autograd.Function):
         if do is None and dstate is None:
             return (None,) * 8
         q, k, v, g, beta, initial, lengths = ctx.saved_tensors
-        ragged = lengths is not None
-        # dense whatever the strides of the inputs; tokens past a row's length are not written by the kernels
-        dq, dk, dv, dg, dbeta = (t.new_zeros(t.shape) if ragged else t.new_empty(t.shape) for t in (q, k, v, g, beta))
+        # dense whatever the strides of the inputs
+        dq, dk, dv, dg, dbeta = (t.new_empty(t.shape) for t in (q, k, v, g, beta))
         do = v.new_zeros(v.shape) if do is None else do.contiguous()
         dstate = None if dstate is None else dstate.contiguous()
         dinitial = initial.new_empty(initial.shape) if ctx.needs_input_grad[5] else None

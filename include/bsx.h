@@ -559,8 +559,8 @@ typedef enum { BSX_T_F32 = 0, BSX_T_BF16 = 1, BSX_T_F16 = 2, BSX_T_EVENT8 = 3, B
  * -infinity: the state is dropped) and beta (batch, tokens, v_heads) float32.  Strides of batch,
  * token and head in elements; the last dimension is dense.  Value head h uses key head
  * h / (v_heads / k_heads).  initial (batch, v_heads, dk, dv) float32, dense; NULL = zero.
- * lengths (batch) int32 device values; NULL = tokens.  A row's tokens from its length on are not
- * read, and its outputs and gradients there are not written.  dk <= 128, dv <= 4096.
+ * lengths (batch) int32 device values, clipped to [0, tokens]; NULL = tokens.  A row's tokens from
+ * its length on are not read, and its outputs and gradients there are set to zero.  dk <= 128, dv <= 4096.
  */
 typedef struct bsx_delta {
   int64_t batch, tokens;
