@@ -40,6 +40,31 @@ __device__ __forceinline__ int quantized(float x, float s, float inv) {
   return (int)fminf(fmaxf(n, -127.f), 127.f);
 }
 
+template <typename E> struct Stretch { E v[16 / sizeof(E)]; };
+
+__device__ __forceinline__ bool note(float x, float& top) {   // true for what is not finite
+  const float a = fabsf(x);
+  top = fmaxf(top, a);
+  return !(a <= 3.402823466e38f);
+}
+
+// Four values in one word.  The nearest integer comes from the sum with 1.5 * 2^23, whose low byte is it; where a value
+// comes near a border the exact rule decides, out of line.
+static __device__ __noinline__ uint32_t four_exact(float4 x, float s, float inv) {
+  return (uint32_t)(uint8_t)(int8_t)quantized(x.x, s, inv) | (uint32_t)(uint8_t)(int8_t)quantized(x.y, s, inv) << 8 |
+         (uint32_t)(uint8_t)(int8_t)quantized(x.z, s, inv) << 16 | (uint32_t)(uint8_t)(int8_t)quantized(x.w, s, inv) << 24;
+}
+__device__ __forceinline__ uint32_t four(float4 x, float s, float inv) {
+  constexpr float M = 12582912.f;
+  const float y0 = x.x * inv, y1 = x.y * inv, y2 = x.z * inv, y3 = x.w * inv;
+  const float t0 = __fadd_rn(y0, M), t1 = __fadd_rn(y1, M), t2 = __fadd_rn(y2, M), t3 = __fadd_rn(y3, M);
+  const float d = fmaxf(fmaxf(fabsf(y0 - __fsub_rn(t0, M)), fabsf(y1 - __fsub_rn(t1, M))),
+                        fmaxf(fabsf(y2 - __fsub_rn(t2, M)), fabsf(y3 - __fsub_rn(t3, M))));
+  if (!(d < 0.4999f)) return four_exact(x, s, inv);
+  return __byte_perm(__byte_perm(__float_as_uint(t0), __float_as_uint(t1), 0x0040),
+                     __byte_perm(__float_as_uint(t2), __float_as_uint(t3), 0x0040), 0x5410);
+}
+
 // Rows of a product's left operand are padded to whole 16-byte stretches.
 inline int64_t padded(int64_t k) { return (k + 15) / 16 * 16; }
 
@@ -79,6 +104,9 @@ struct Plan { int rows, splits; };
 
 bool few_applies(int64_t M, int64_t N, int64_t Kp);
 int launch_few(const Product& p, int dtype, cudaStream_t st);
+// Rows that are not quantised yet, by the same kernel (p.x and p.sx unused).
+bool few_takes_rows(int64_t M, int64_t K);
+int launch_few_rows(const Product& p, const void* x, int format, int64_t stride, int64_t K, int dtype, cudaStream_t st);
 Plan plan_tiles(int64_t M, int64_t N, int64_t Kp, int sms);
 int launch_tiles(const Product& p, Plan plan, int dtype, cudaStream_t st);
 

@@ -9,31 +9,6 @@ namespace int8 {
 
 constexpr int kHeld = 2;   // 16-byte stretches a thread keeps between the two passes over its row
 
-template <typename E> struct Stretch { E v[16 / sizeof(E)]; };
-
-__device__ __forceinline__ bool note(float x, float& top) {   // true for what is not finite
-  const float a = fabsf(x);
-  top = fmaxf(top, a);
-  return !(a <= 3.402823466e38f);
-}
-
-// Four values in one word.  The nearest integer comes from the sum with 1.5 * 2^23, whose low byte is it; where a value
-// comes near a border the exact rule decides, out of line.
-__device__ __noinline__ uint32_t four_exact(float4 x, float s, float inv) {
-  return (uint32_t)(uint8_t)(int8_t)quantized(x.x, s, inv) | (uint32_t)(uint8_t)(int8_t)quantized(x.y, s, inv) << 8 |
-         (uint32_t)(uint8_t)(int8_t)quantized(x.z, s, inv) << 16 | (uint32_t)(uint8_t)(int8_t)quantized(x.w, s, inv) << 24;
-}
-__device__ __forceinline__ uint32_t four(float4 x, float s, float inv) {
-  constexpr float M = 12582912.f;
-  const float y0 = x.x * inv, y1 = x.y * inv, y2 = x.z * inv, y3 = x.w * inv;
-  const float t0 = __fadd_rn(y0, M), t1 = __fadd_rn(y1, M), t2 = __fadd_rn(y2, M), t3 = __fadd_rn(y3, M);
-  const float d = fmaxf(fmaxf(fabsf(y0 - __fsub_rn(t0, M)), fabsf(y1 - __fsub_rn(t1, M))),
-                        fmaxf(fabsf(y2 - __fsub_rn(t2, M)), fabsf(y3 - __fsub_rn(t3, M))));
-  if (!(d < 0.4999f)) return four_exact(x, s, inv);
-  return __byte_perm(__byte_perm(__float_as_uint(t0), __float_as_uint(t1), 0x0040),
-                     __byte_perm(__float_as_uint(t2), __float_as_uint(t3), 0x0040), 0x5410);
-}
-
 // One block per row: the maximum, then the values.  Bound by reading the row once and writing a byte per entry; the first
 // kHeld 16-byte stretches of a thread stay in registers in between, the rest comes from L2 the second time.
 template <typename E, bool VEC, int THREADS>
@@ -328,7 +303,7 @@ extern "C" int bsx_int8_matmul(const int8_t* q, const float* scale, const int8_t
 }
 
 extern "C" size_t bsx_int8_dense_workspace_bytes(int64_t M, int64_t K, int64_t N) {
-  if (check_sizes(M, K, N) != BSX_OK) return 0;
+  if (check_sizes(M, K, N) != BSX_OK || few_takes_rows(M, K)) return 0;
   return aligned((size_t)M * padded(K)) + aligned((size_t)M * sizeof(float)) + partial_bytes(M, K, N, sm_count());
 }
 
@@ -345,6 +320,12 @@ extern "C" int bsx_int8_dense(const void* x, int format, int64_t row_stride, con
   if (!aligned16(wq)) return fail(BSX_ERR_INVALID_ARG, "8-bit operands must start on a 16-byte boundary");
   const int sms = sm_count();
   if (sms <= 0) return fail(BSX_ERR_CUDA, "no CUDA device");
+  if (few_takes_rows(M, K)) {     // one kernel, no workspace
+    Product p = {};
+    p.w = wq; p.sw = wscale; p.out = out;
+    p.M = M; p.N = N; p.Kp = padded(K);
+    return launch_few_rows(p, x, format, row_stride, K, out_dtype, as_stream(stream));
+  }
   const size_t qb = aligned((size_t)M * padded(K)), sb = aligned((size_t)M * sizeof(float));
   if (!ws || !aligned16(ws) || ws_bytes < qb + sb + partial_bytes(M, K, N, sms))
     return fail(BSX_ERR_WORKSPACE, "workspace missing, misaligned or too small");

@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(THREADS, 1) backward_scan_kernel(Args a, int g
       clear(ah[n]);
       clear(al[n]);
     }
-#pragma unroll 2
+#pragma unroll
     for (int ks = 0; ks < 8; ++ks) {
       float hi[4], lo[4];
       float2 kk[NT];

@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(Args a, int groups, in
       clear(zh[e]);
       clear(zl[e]);
     }
-#pragma unroll 8
+#pragma unroll
     for (int ks = 0; ks < DK / 8; ++ks) {
       float hi[4], lo[4];
       get_split(gS, ks, lane, hi, lo);

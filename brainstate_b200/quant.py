@@ -42,10 +42,11 @@ def _rows(x, n: Optional[int]):
     lead, n = tuple(t.shape[:-1]), t.shape[-1]
     if n == 0:
         raise ValueError('rows without entries cannot be quantised')
-    x2 = t.reshape(-1, n) if t.numel() else t.new_empty((0 if 0 in lead else 1, n))
-    if n > 1 and x2.stride(-1) != 1:
-        x2 = x2.contiguous()
-    return x2, kinds[t.dtype], lead
+    if len(lead) != 1:
+        t = t.reshape(-1, n) if t.numel() else t.new_empty((0, n))
+    if n > 1 and t.stride(-1) != 1:
+        t = t.contiguous()
+    return t, kinds[t.dtype], lead
 
 
 class Int8Rows:
@@ -136,12 +137,13 @@ def int8_matmul(x, w: Int8Dense, out_dtype: Optional[torch.dtype] = None) -> tor
     else:
         data, fmt, lead = _rows(x, n_pre)
         kind = torch.float32 if fmt >= _lib.T_EVENT8 else data.dtype
-    kind = kind if out_dtype is None else out_dtype
-    if kind not in _TYPES:
-        raise TypeError(f'out_dtype must be float32, bfloat16 or float16, got {kind}')
-    if data.get_device() != w.q.get_device():
-        raise ValueError(f'input is on {data.device}, the weights on {w.q.device}')
+    if out_dtype is not None:
+        kind = out_dtype
+        if kind not in _TYPES:
+            raise TypeError(f'out_dtype must be float32, bfloat16 or float16, got {kind}')
     m, dev = data.shape[0], data.get_device()
+    if dev != w.q.get_device():
+        raise ValueError(f'input is on {data.device}, the weights on {w.q.device}')
     out = data.new_empty(lead + (n_post,), dtype=kind)
     if rows:
         n = lib().bsx_int8_matmul_workspace_bytes(m, n_pre, n_post)
@@ -150,7 +152,7 @@ def int8_matmul(x, w: Int8Dense, out_dtype: Optional[torch.dtype] = None) -> tor
                 n_post, out.data_ptr(), _TYPES[kind], None if ws is None else ws.data_ptr(), n)
     else:
         n = lib().bsx_int8_dense_workspace_bytes(m, n_pre, n_post)
-        ws = w.q.new_empty(n)
+        ws = w.q.new_empty(n) if n else None
         call_on(dev, lib().bsx_int8_dense, data.data_ptr(), fmt, data.stride(0), w.q.data_ptr(), w.scale.data_ptr(), m, n_pre,
-                n_post, out.data_ptr(), _TYPES[kind], ws.data_ptr(), n)
+                n_post, out.data_ptr(), _TYPES[kind], None if ws is None else ws.data_ptr(), n)
     return out

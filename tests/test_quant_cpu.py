@@ -26,7 +26,7 @@ def test_library_refusals_need_no_gpu(bsx):
     assert rows(k=131073) == BSX_ERR_UNSUPPORTED and rows(m=0) == 0
     cols = lambda w=at, kind=0, k=8, n=8: bsx.bsx_int8_quantize_weights(w, kind, k, n, at, at, None)
     assert cols(w=None) == cols(kind=3) == BSX_ERR_INVALID_ARG and cols(k=0) == BSX_ERR_UNSUPPORTED and cols(n=0) == 0
-    assert bsx.bsx_int8_dense_workspace_bytes(4, 100, 8) >= 4 * 112 + 16
+    assert bsx.bsx_int8_dense_workspace_bytes(5, 100, 8) >= 5 * 112 + 20
     assert bsx.bsx_int8_dense_workspace_bytes(4, 200000, 8) == 0
 
 

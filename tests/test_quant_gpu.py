@@ -33,8 +33,10 @@ def close(y, want, dtype):
     assert bool((((y - want).abs() <= step * 1.001 * want.abs() + least) | torch.isnan(want)).all())
 
 
-# rows on both sides of every change of kernel and tile (8, 16, 24, 32 | tiles of 128), channels likewise
-SIZES = [(1, 16, 1), (1, 1000, 17), (7, 64, 16), (8, 100, 33), (9, 4096, 70), (16, 31, 16), (17, 1, 40), (24, 640, 48),
+# rows on both sides of every change of kernel and tile (4, 8, 16, 24, 32 | 64, 128, 256), channels likewise; rows that a
+# product's blocks quantise themselves (up to 4 x 40704 bytes in all)
+SIZES = [(2, 1000, 40), (3, 8192, 33), (3, 77, 64), (4, 4096, 100), (4, 10176, 20), (4, 10192, 20), (1, 40704, 16), (1, 40720, 17),
+         (5, 513, 30), (1, 16, 1), (1, 1000, 17), (7, 64, 16), (8, 100, 33), (9, 4096, 70), (16, 31, 16), (17, 1, 40), (24, 640, 48),
          (31, 257, 100), (32, 2048, 65), (33, 64, 64), (64, 500, 129), (127, 128, 256), (128, 129, 255), (129, 4096, 300),
          (100, 8192, 520), (40, 16000, 64), (200, 1001, 777), (1000, 96, 1000)]
 
