@@ -43,26 +43,26 @@ __global__ void __launch_bounds__(128) prepare_kernel(Args a) {
   const int rows = (int)min((int64_t)kC, len - t0);
   const int64_t ci = (int64_t)bh * a.NC + chunk;
 
+  // g and beta first: their sums are a chain that starts with these loads
+  float gv[2] = {0.f, 0.f}, bv[2] = {0.f, 0.f};
+  if (warp == 0) {
+    const float* gp = a.g + b * a.gs[0] + t0 * a.gs[1] + h * a.gs[2];
+    const float* bp = a.beta + b * a.bs[0] + t0 * a.bs[1] + h * a.bs[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (2 * lane + e < rows) {
+        gv[e] = gp[(2 * lane + e) * a.gs[1]];
+        bv[e] = bp[(2 * lane + e) * a.bs[1]];
+      }
+  }
   const E* kp = static_cast<const E*>(a.k) + b * a.ks[0] + t0 * a.ks[1] + hk * a.ks[2];
   const E* qp = static_cast<const E*>(a.q) + b * a.qs[0] + t0 * a.qs[1] + hk * a.qs[2];
   stage(sk, L::PK, kp, a.ks[1], rows, a.dk, DK, a.vec_qk, tid, 128);
   stage(sq, L::PK, qp, a.qs[1], rows, a.dk, DK, a.vec_qk, tid, 128);
   cp_commit();
   if (warp == 0) {  // sums of g: two tokens a lane, then across the lanes
-    const float* gp = a.g + b * a.gs[0] + t0 * a.gs[1] + h * a.gs[2];
-    const float* bp = a.beta + b * a.bs[0] + t0 * a.bs[1] + h * a.bs[2];
-    double x0 = 0, x1 = 0;
-    float b0 = 0.f, b1 = 0.f;
-    if (2 * lane < rows) {
-      const float v = gp[(2 * lane) * a.gs[1]];
-      x0 = v < -128.f ? -128.f : v;
-      b0 = bp[(2 * lane) * a.bs[1]];
-    }
-    if (2 * lane + 1 < rows) {
-      const float v = gp[(2 * lane + 1) * a.gs[1]];
-      x1 = v < -128.f ? -128.f : v;
-      b1 = bp[(2 * lane + 1) * a.bs[1]];
-    }
+    const double x0 = gv[0] < -128.f ? -128.f : gv[0], x1 = gv[1] < -128.f ? -128.f : gv[1];
+    const float b0 = bv[0], b1 = bv[1];
     double s = x0 + x1;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -84,44 +84,43 @@ __global__ void __launch_bounds__(128) prepare_kernel(Args a) {
     *reinterpret_cast<float2*>(vec + 4 * kC + 2 * lane) = make_float2(l0, l1);
   }
   cp_wait<0>();
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncthreads();
-  if (h % (a.Hv / a.Hk) == 0) {   // both tiles as they lie here: later kernels take them with one copy
-    int4* kq = static_cast<int4*>(a.kq) + (((int64_t)b * a.Hk + hk) * a.NC + chunk) * (2 * L::tile / 16);
-    for (int i = tid; i < (int)(2 * L::tile / 16); i += 128) kq[i] = reinterpret_cast<const int4*>(smem)[i];
+  const bool packs = tid == 0 && h % (a.Hv / a.Hk) == 0;
+  if (packs) {   // both tiles as they lie here, in one copy: later kernels take them with one copy too
+    unsigned char* kq = static_cast<unsigned char*>(a.kq) + (((int64_t)b * a.Hk + hk) * a.NC + chunk) * (2 * L::tile);
+    bulk_s2g(kq, smem, (uint32_t)(2 * L::tile));
   }
 
-  // rows 16 * warp .. + 15 of K K^T and Q K^T, tiles on and below the diagonal
-  float kk[8][4], qk[8][4];
+  // K K^T and Q K^T: the 20 tiles (16 x 8) on and below the diagonal by rows, five to a warp
+  float kk[5][4], qk[5][4];
+  int r0[5], nt[5];       // first row (of this lane) and column tile
 #pragma unroll
-  for (int n = 0; n < 8; ++n)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) kk[n][i] = qk[n][i] = 0.f;
-  const int r0 = warp * 16 + g;
+  for (int u = 0; u < 5; ++u) {
+    const int i = 5 * warp + u, r = i < 2 ? 0 : i < 6 ? 1 : i < 12 ? 2 : 3;
+    nt[u] = i - r * (r + 1);
+    r0[u] = r * 16 + g;
+    clear(kk[u]);
+    clear(qk[u]);
+  }
+#pragma unroll 2
   for (int ks = 0; ks < DK / 8; ++ks) {
     const int c = ks * 8 + 2 * t;
-    const float2 k0 = pair(sk + r0 * L::PK + c), k1 = pair(sk + (r0 + 8) * L::PK + c);
-    const float2 q0 = pair(sq + r0 * L::PK + c), q1 = pair(sq + (r0 + 8) * L::PK + c);
-    float ak[4] = {k0.x, k1.x, k0.y, k1.y}, aq[4] = {q0.x, q1.x, q0.y, q1.y};
-    float akl[4], aql[4], akh[4], aqh[4];
-    if (!IsExact<E>::value) {
-      split4(ak, akh, akl);
-      split4(aq, aqh, aql);
-    }
 #pragma unroll
-    for (int n0 = 0; n0 < 8; n0 += 2) {
-      if (n0 > 2 * warp) break;
-      float2 bb[2];
-#pragma unroll
-      for (int n = 0; n < 2; ++n) bb[n] = pair(sk + ((n0 + n) * 8 + g) * L::PK + c);
+    for (int u = 0; u < 5; ++u) {
+      const float2 k0 = pair(sk + r0[u] * L::PK + c), k1 = pair(sk + (r0[u] + 8) * L::PK + c);
+      const float2 q0 = pair(sq + r0[u] * L::PK + c), q1 = pair(sq + (r0[u] + 8) * L::PK + c);
+      const float ak[4] = {k0.x, k1.x, k0.y, k1.y}, aq[4] = {q0.x, q1.x, q0.y, q1.y};
+      const float2 bb = pair(sk + (nt[u] * 8 + g) * L::PK + c);
       if (IsExact<E>::value) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          mma(kk[n0 + n], ak, bb[n].x, bb[n].y);
-          mma(qk[n0 + n], aq, bb[n].x, bb[n].y);
-        }
+        mma(kk[u], ak, bb.x, bb.y);
+        mma(qk[u], aq, bb.x, bb.y);
       } else {
-        mma_split<false, 2>(kk + n0, akh, akl, bb);
-        mma_split<false, 2>(qk + n0, aqh, aql, bb);
+        float h[4], l[4];
+        split4(ak, h, l);
+        mma_split<false, 1>(kk + u, h, l, &bb);
+        split4(aq, h, l);
+        mma_split<false, 1>(qk + u, h, l, &bb);
       }
     }
   }
@@ -129,26 +128,25 @@ __global__ void __launch_bounds__(128) prepare_kernel(Args a) {
   float* Pm = Tm + kTri;
   float* Bm = BACK ? a.Bm + ci * kTri : nullptr;
 #pragma unroll
-  for (int n = 0; n < 8; ++n) {
-    if (n > 2 * warp + 1) break;
+  for (int u = 0; u < 5; ++u)
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
-      const int i = r0 + 8 * hf, j = n * 8 + 2 * t;
+      const int i = r0[u] + 8 * hf, n = nt[u], j = n * 8 + 2 * t;
       float p[2], m[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float gam = j + e <= i ? expf((sHi[i] - sHi[j + e]) + (sLo[i] - sLo[j + e])) : 0.f;
-        p[e] = j + e <= i ? a.scale * gam * qk[n][2 * hf + e] : 0.f;
-        m[e] = j + e < i ? gam * kk[n][2 * hf + e] : 0.f;
+        p[e] = j + e <= i ? a.scale * gam * qk[u][2 * hf + e] : 0.f;
+        m[e] = j + e < i ? gam * kk[u][2 * hf + e] : 0.f;
         sA[i * L::PA + j + e] = sBeta[i] * m[e];
       }
-      if (n <= 2 * warp + hf) {
-        const int at = tri(2 * warp + hf, n) + lane * 2;
+      if (n <= i >> 3) {
+        const int at = tri(i >> 3, n) + lane * 2;
         *reinterpret_cast<float2*>(Pm + at) = make_float2(p[0], p[1]);
         if (BACK) *reinterpret_cast<float2*>(Bm + at) = make_float2(m[0], m[1]);
       }
     }
-  }
+  if (packs) bulk_read_wait();    // T takes the tiles' place
   __syncthreads();
 
   // diagonal blocks of T: lane j solves column j of block `warp`
@@ -157,13 +155,19 @@ __global__ void __launch_bounds__(128) prepare_kernel(Args a) {
     const float* Ad = sA + (16 * warp) * L::PA + 16 * warp;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      float v = i == lane ? 1.f : 0.f;
+      float r[16];
 #pragma unroll
-      for (int l = 0; l < 16; ++l)
-        if (l < i) v = fmaf(-Ad[i * L::PA + l], x[l], v);
-      x[i] = v;
-      sT[(16 * warp + i) * L::PA + 16 * warp + lane] = v;
+      for (int l = 0; l < i; l += 4) *reinterpret_cast<float4*>(r + l) = *reinterpret_cast<const float4*>(Ad + i * L::PA + l);
+      float v = i == lane ? 1.f : 0.f, u = 0.f;     // two chains
+#pragma unroll
+      for (int l = 0; l < i; ++l) {
+        if (l & 1) u = fmaf(-r[l], x[l], u);
+        else v = fmaf(-r[l], x[l], v);
+      }
+      x[i] = v + u;
     }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sT[(16 * warp + i) * L::PA + 16 * warp + lane] = x[i];
   }
   __syncwarp();
   // -T_ii A_il for l < i = warp, kept as left operands
