@@ -56,13 +56,13 @@ def compare(got, want):
 
 
 @pytest.mark.parametrize('dtype', [F32, BF16, F16])
-@pytest.mark.parametrize('T', [1, 2, 16, 17, 63, 64, 65, 200])
+@pytest.mark.parametrize('T', [1, 2, 8, 9, 16, 63, 64, 65, 200])
 def test_lengths(cuda, dtype, T):
     compare(*run_both(inputs(2, T, 2, 2, 64, 48, dtype, seed=T)))
 
 
 @pytest.mark.parametrize('dtype', [F32, BF16, F16])
-@pytest.mark.parametrize('dk,dv', [(1, 1), (16, 20), (33, 100), (64, 16), (65, 33), (100, 192), (128, 128), (128, 300)])
+@pytest.mark.parametrize('dk,dv', [(1, 1), (16, 20), (33, 100), (64, 16), (65, 33), (100, 192), (128, 128), (128, 300), (8, 1100)])
 def test_sizes(cuda, dtype, dk, dv):
     compare(*run_both(inputs(1, 150, 1, 2, dk, dv, dtype, seed=dk)))
 
@@ -75,7 +75,7 @@ def test_heads_and_batches(cuda, dtype, B, Hk, Hv, dk):
 
 
 @pytest.mark.parametrize('dtype', [F32, BF16])
-@pytest.mark.parametrize('T', [9, 130])
+@pytest.mark.parametrize('T', [7, 9, 130])
 def test_padded_rows(cuda, dtype, T):
     """What lies behind a row's length is not read (it holds NaN and infinities here), and comes out as zero."""
     args = inputs(5, T, 2, 4, 48, 40, dtype, seed=T)
@@ -101,7 +101,7 @@ def test_lengths_out_of_range_are_clipped(cuda):
         assert torch.equal(x, y)
 
 
-@pytest.mark.parametrize('T', [10, 140])
+@pytest.mark.parametrize('T', [7, 10, 140])
 def test_full_decay_and_no_learning(cuda, T):
     """g = -inf drops the state, large decays and beta = 0 and 1 in between; nothing turns into NaN."""
     args = inputs(2, T, 1, 2, 32, 32, F32, seed=3)
@@ -121,6 +121,46 @@ def test_alike_keys(cuda):
     """Keys of a chunk that are nearly the same: (I + A)^{-1} must not be summed as a power series."""
     args = inputs(1, 128, 1, 1, 64, 64, F32, seed=8, alike=6.0)
     compare(*run_both(args))
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_long_sequence(cuda, dtype):
+    """3000 tokens (47 chunks) with slow decay: errors must not pile up from chunk to chunk."""
+    args = inputs(1, 3000, 1, 2, 16, 16, dtype, seed=12)
+    args['g'] *= 0.05
+    compare(*run_both(args))
+
+
+def test_many_rows_of_different_length(cuda):
+    """More chunks than the reverse kernel has blocks, most rows short: chunks are handed out as blocks become free."""
+    args = inputs(60, 200, 2, 4, 16, 16, F32, seed=9)
+    compare(*run_both(args, [(7 * b) % 201 if b % 3 else b % 5 for b in range(60)]))
+
+
+def test_two_streams_at_once(cuda):
+    """Two calls in flight with workspaces of their own, rows of different length among them."""
+    from brainstate_b200 import plastic
+    sets = []
+    for seed in (1, 2):
+        a = {n: x.cuda() for n, x in inputs(9, 260, 2, 4, 64, 64, BF16, seed=seed).items()}
+        sets.append((a.pop('initial'), [x.requires_grad_(True) for x in a.values()],
+                     torch.arange(9, device='cuda', dtype=torch.int32) * 32))
+
+    def once(initial, leaves, lengths):
+        o, s = plastic.delta_rule(*leaves, initial_state=initial, lengths=lengths)
+        return (o, s) + torch.autograd.grad(o.float().square().sum() + s.sum(), leaves)
+
+    want = [once(*x) for x in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(5):
+        got = []
+        for st, x in zip(streams, sets):
+            with torch.cuda.stream(st):
+                got.append(once(*x))
+        torch.cuda.synchronize()
+        for x, y in zip(got, want):
+            assert all(torch.equal(p, q) for p, q in zip(x, y))
 
 
 def test_zero_tokens_and_empty_batch(cuda):
