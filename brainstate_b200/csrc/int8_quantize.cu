@@ -119,48 +119,73 @@ event_rows_kernel(const void* __restrict__ x, int64_t stride, int64_t M, int64_t
   }
 }
 
-// Weights (K, N): 32 columns a block, eight rows of threads; the maxima, then 32 x 32 tiles turned through shared memory.
+// Weights (K, N), 32 columns a block: the maxima over a range of rows, met in `top` as the bits of non-negative floats
+// (infinity for what is not finite) ...
+template <typename E>
+__global__ void __launch_bounds__(256) column_top_kernel(const E* __restrict__ w, int64_t K, int64_t N, uint32_t* __restrict__ top) {
+  __shared__ float part[8][32];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int64_t n = (int64_t)blockIdx.x * 32 + tx;
+  float t = 0.f;
+  bool bad = false;
+  if (n < N)
+#pragma unroll 4
+    for (int64_t k = (int64_t)blockIdx.y * 8 + ty; k < K; k += (int64_t)gridDim.y * 8) bad |= note(to_f<E>(w[k * N + n]), t);
+  part[ty][tx] = bad ? __int_as_float(0x7f800000) : t;
+  __syncthreads();
+  if (ty == 0 && n < N) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t = fmaxf(t, part[i][tx]);
+    atomicMax(top + n, __float_as_uint(t));
+  }
+}
+
+// ... then tiles of 128 rows, turned through shared memory ...
 template <typename E>
 __global__ void __launch_bounds__(256)
 quantize_columns_kernel(const E* __restrict__ w, int64_t K, int64_t N, int64_t Kp, int8_t* __restrict__ q,
-                        float* __restrict__ scale) {
-  __shared__ float top_s[8][32];
-  __shared__ int bad_s[32];
-  __shared__ int8_t tile[32][36];
+                        const uint32_t* __restrict__ top) {
+  __shared__ int8_t tile[32][132];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int64_t n0 = (int64_t)blockIdx.x * 32, n = n0 + tx;
-  if (ty == 0) bad_s[tx] = 0;
-  __syncthreads();
-  float top = 0.f;
-  bool bad = false;
-  if (n < N)
-    for (int64_t k = ty; k < K; k += 8) {
-      const float a = fabsf(to_f<E>(w[k * N + n]));
-      bad |= !(a <= 3.402823466e38f);
-      top = fmaxf(top, a);
-    }
-  top_s[ty][tx] = top;
-  if (bad) bad_s[tx] = 1;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = fmaxf(top, top_s[i][tx]);
-  const bool finite = bad_s[tx] == 0;
-  const float s = scale_of(top, finite);
-  if (ty == 0 && n < N) scale[n] = s;
-  const bool zero = !finite || s == 0.f;
+  const int64_t n0 = (int64_t)blockIdx.x * 32, n = n0 + tx, k0 = (int64_t)blockIdx.y * 128;
+  const float t = n < N ? __uint_as_float(top[n]) : 0.f;
+  const float s = scale_of(t, t <= 3.402823466e38f);
+  const bool zero = !(s > 0.f);
   const float inv = s < 1e-30f ? __int_as_float(0x7fffffff) : 1.f / s;
-  for (int64_t k0 = 0; k0 < Kp; k0 += 32) {
+#pragma unroll 4
+  for (int i = 0; i < 16; ++i) {
+    const int64_t k = k0 + ty + 8 * i;
+    tile[tx][ty + 8 * i] = (n < N && k < K && !zero) ? (int8_t)quantized(to_f<E>(w[k * N + n]), s, inv) : (int8_t)0;
+  }
+  __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t k = k0 + ty + 8 * i;
-      tile[tx][ty + 8 * i] = (n < N && k < K && !zero) ? (int8_t)quantized(to_f<E>(w[k * N + n]), s, inv) : (int8_t)0;
-    }
-    __syncthreads();
-    const int r = threadIdx.x >> 3, c = (threadIdx.x & 7) * 4;
+  for (int i = 0; i < 4; ++i) {
+    const int r = ty + 8 * i, c = tx * 4;
     if (n0 + r < N && k0 + c < Kp)
       *reinterpret_cast<uint32_t*>(q + (n0 + r) * Kp + k0 + c) = *reinterpret_cast<const uint32_t*>(&tile[r][c]);
-    __syncthreads();
   }
+}
+
+// ... and the maxima become scales.
+__global__ void __launch_bounds__(256) column_scale_kernel(float* scale, int64_t N) {
+  const int64_t n = blockIdx.x * 256ll + threadIdx.x;
+  if (n < N) scale[n] = scale_of(scale[n], scale[n] <= 3.402823466e38f);
+}
+
+template <typename E>
+static int launch_columns(const void* w, int64_t K, int64_t N, int8_t* q, float* scale, cudaStream_t st) {
+  const E* p = static_cast<const E*>(w);
+  const int64_t Kp = padded(K), cols = (N + 31) / 32, want = 8ll * sm_count() / cols + 1, most = (K + 63) / 64;
+  BSX_CUDA(cudaMemsetAsync(scale, 0, N * sizeof(float), st));
+  column_top_kernel<E><<<dim3((unsigned)cols, (unsigned)(want < most ? want : most)), 256, 0, st>>>(
+      p, K, N, reinterpret_cast<uint32_t*>(scale));
+  BSX_LAUNCH_CHECK("column_top_kernel");
+  quantize_columns_kernel<E><<<dim3((unsigned)cols, (unsigned)((Kp + 127) / 128)), 256, 0, st>>>(
+      p, K, N, Kp, q, reinterpret_cast<const uint32_t*>(scale));
+  BSX_LAUNCH_CHECK("quantize_columns_kernel");
+  column_scale_kernel<<<(unsigned)((N + 255) / 256), 256, 0, st>>>(scale, N);
+  BSX_LAUNCH_CHECK("column_scale_kernel");
+  return BSX_OK;
 }
 
 template <typename E, bool VEC>
@@ -267,16 +292,9 @@ extern "C" int bsx_int8_quantize_weights(const void* w, int dtype, int64_t K, in
   if (!aligned16(q)) return fail(BSX_ERR_INVALID_ARG, "q must start on a 16-byte boundary");
   if (sm_count() <= 0) return fail(BSX_ERR_CUDA, "no CUDA device");
   cudaStream_t st = as_stream(stream);
-  const unsigned grid = (unsigned)((N + 31) / 32);
-  const int64_t Kp = padded(K);
-  if (dtype == BSX_T_F32)
-    quantize_columns_kernel<float><<<grid, 256, 0, st>>>(static_cast<const float*>(w), K, N, Kp, q, scale);
-  else if (dtype == BSX_T_BF16)
-    quantize_columns_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(w), K, N, Kp, q, scale);
-  else
-    quantize_columns_kernel<__half><<<grid, 256, 0, st>>>(static_cast<const __half*>(w), K, N, Kp, q, scale);
-  BSX_LAUNCH_CHECK("quantize_columns_kernel");
-  return BSX_OK;
+  if (dtype == BSX_T_F32) return launch_columns<float>(w, K, N, q, scale, st);
+  if (dtype == BSX_T_BF16) return launch_columns<__nv_bfloat16>(w, K, N, q, scale, st);
+  return launch_columns<__half>(w, K, N, q, scale, st);
 }
 
 extern "C" size_t bsx_int8_matmul_workspace_bytes(int64_t M, int64_t K, int64_t N) {

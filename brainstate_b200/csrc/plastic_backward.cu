@@ -783,6 +783,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1) backward_chunk_kernel(Args a
         dqa[m][n][i] *= a.scale * eG[r];
         d1[m][n][i] = fmaf(-beta[r] * eG[r], d1[m][n][i], eD[r] * d3[m][n][i]);
       }
+  // sums of their own, added in one rounding
+  float (*ek)[N][4] = d3;      // E^T Q + (F + F^T) K
+  float eq[2][N][4];           // E K
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      clear(ek[m][n]);
+      clear(eq[m][n]);
+    }
 #pragma unroll 2
   for (int ks = 0; ks < 8; ++ks) {
     const int c0 = ks * 8 + 2 * t;
@@ -813,23 +823,32 @@ __global__ void __launch_bounds__(kChunkThreads, 1) backward_chunk_kernel(Args a
         const float2 p0 = pair(sE + i * L::PE + c0), p1 = pair(sE + (i + 8) * L::PE + c0);
         const float x[4] = {p0.x, p1.x, p0.y, p1.y};
         prepare(x);
-        product(dqa[m], kk);
+        product(eq[m], kk);
       }
       if (ks * 8 + 7 >= i0) {
         const float* et = sE + c0 * L::PE + i;
         const float x[4] = {et[0], et[8], et[L::PE], et[L::PE + 8]};
         prepare(x);
-        product(d1[m], qq);
+        product(ek[m], qq);
       }
       {
         const float2 f0 = pair(sF + i * L::PE + c0), f1 = pair(sF + (i + 8) * L::PE + c0);
         const float* ft = sF + c0 * L::PE + i;
         const float x[4] = {f0.x + ft[0], f1.x + ft[8], f0.y + ft[L::PE], f1.y + ft[L::PE + 8]};
         prepare(x);
-        product(d1[m], kk);
+        product(ek[m], kk);
       }
     }
   }
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        dqa[m][n][i] += eq[m][n][i];
+        d1[m][n][i] += ek[m][n][i];
+      }
   __syncthreads();      // K, Q, E and F are free
   if (tid == 0 && next < items) load_chunk(next);
   auto finish = [&](auto* dq, auto* dk, int heads, int ho) {
