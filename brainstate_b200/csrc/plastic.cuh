@@ -10,9 +10,11 @@
 //
 // Products run on tf32 tensor instructions (16x8x8, 32-bit sums).  bf16 and fp16 values are exact in tf32; a 32-bit
 // operand is split into hi + lo tf32 parts (22 bits), so a product with one 16-bit operand takes two instructions
-// and one of two 32-bit operands three (lo x lo, 2^-22 of the product, is dropped).  Everything the state, its
-// cotangent and the gate gradients depend on is computed this way; only the last product before a bf16 output uses
-// the hi parts alone (2^-12 before a rounding of 2^-9).
+// and one of two 32-bit operands three (lo x lo, 2^-22 of the product, is dropped).  The products with bf16 keys and
+// queries that carry the state run on bf16 instructions instead (16x8x16, the same time for twice the depth): the 32-bit
+// operand is then three bf16 parts (24 bits), three instructions where tf32 takes four, and the bf16 operand goes in as
+// it lies in memory.  Everything the state, its cotangent and the gate gradients depend on is computed this way; only
+// products that go straight into a bf16 output take fewer parts (2^-12 or 2^-17 before a rounding of 2^-9).
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -196,6 +198,68 @@ __device__ __forceinline__ void get_split(const float4* base, int tile, int lane
   const float4 x = base[tile * 64 + lane], y = base[tile * 64 + 32 + lane];
   hi[0] = x.x; hi[1] = x.y; hi[2] = x.z; hi[3] = x.w;
   lo[0] = y.x; lo[1] = y.y; lo[2] = y.z; lo[3] = y.w;
+}
+
+// The same in three bf16 parts, two tiles (16 inner entries) together: 1.5 KB, each part the four registers of a left
+// operand of the bf16 instruction (first tile in .x .y, second in .z .w).
+struct Parts { uint32_t w[3]; };     // a pair of neighbouring entries
+__device__ __forceinline__ Parts parts_of(float x0, float x1) {
+  Parts p;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p.w[i]) : "f"(x1), "f"(x0));
+    if (i < 2) {
+      x0 -= __uint_as_float(p.w[i] << 16);
+      x1 -= __uint_as_float(p.w[i] & 0xffff0000u);
+    }
+  }
+  return p;
+}
+__device__ __forceinline__ void put_parts(float4* base, int tile, int lane, const float* c) {
+  const Parts a = parts_of(c[0], c[1]), b = parts_of(c[2], c[3]);
+  uint2* o = reinterpret_cast<uint2*>(base + (tile >> 1) * 96 + lane) + (tile & 1);
+#pragma unroll
+  for (int i = 0; i < 3; ++i) o[i * 64] = make_uint2(a.w[i], b.w[i]);
+}
+__device__ __forceinline__ uint4 get_part(const float4* base, int pair, int part, int lane) {
+  return reinterpret_cast<const uint4*>(base)[pair * 96 + part * 32 + lane];
+}
+__device__ __forceinline__ void mma16(float* c, const uint4& a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+// s^T times the transposed (token, key row) tile X for token tiles own[0], own[1], s in parts: large and small sums; only
+// the first two parts with TWO.
+template <int DK, int PK, bool TWO>
+__device__ __forceinline__ void state_times(float (*h)[4], float (*l)[4], const uint4* a, const __nv_bfloat16* X, int kp,
+                                            const int* own, int g, int t) {
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const uint32_t* x = reinterpret_cast<const uint32_t*>(X + (own[e] * 8 + g) * PK + kp * 16) + t;
+    const uint32_t b0 = x[0], b1 = x[4];
+    if (!TWO) mma16(l[e], a[2], b0, b1);
+    mma16(l[e], a[1], b0, b1);
+    mma16(h[e], a[0], b0, b1);
+  }
+}
+// u (16 tokens of it, in parts) times tiles n = 0 .. N - 1 of a (token, key row) tile at `at`.
+template <int N, int PK>
+__device__ __forceinline__ void update_state(float (*h)[4], float (*l)[4], const uint4* a, const __nv_bfloat16* at, int lane) {
+  const int row = (lane & 7) + ((lane >> 3) & 1) * 8;
+#pragma unroll
+  for (int n = 0; n < N; n += 2) {
+    uint32_t r[4];
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(smem_u32(at + row * PK + n * 8 + (lane >> 4) * 8)) : "memory");
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      mma16(l[n + m], a[2], r[2 * m], r[2 * m + 1]);
+      mma16(l[n + m], a[1], r[2 * m], r[2 * m + 1]);
+      mma16(h[n + m], a[0], r[2 * m], r[2 * m + 1]);
+    }
+  }
 }
 
 // Right-operand tiles from a (row, column) tile in shared memory: N 8x8 tiles whose rows are the outer index (pairs of

@@ -117,6 +117,7 @@ template <typename E, int DK, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1) backward_scan_kernel(Args a, int groups, int stages) {
   using L = BackScanLayout<E, DK>;
   constexpr bool X = IsExact<E>::value;
+  constexpr bool B16 = std::is_same<E, __nv_bfloat16>::value;
   constexpr int DKW = DK / 4, NT = DKW / 8;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ __align__(8) uint64_t bars[2];
@@ -188,7 +189,10 @@ __global__ void __launch_bounds__(THREADS, 1) backward_scan_kernel(Args a, int g
                 make_float2(s[n][2 * hf], s[n][2 * hf + 1]);
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n) put_split(gS, w * NT + n, lane, s[n]);
+    for (int n = 0; n < NT; ++n) {
+      if constexpr (B16) put_parts(gS, w * NT + n, lane, s[n]);
+      else put_split(gS, w * NT + n, lane, s[n]);
+    }
     float x[2][4];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -206,13 +210,21 @@ __global__ void __launch_bounds__(THREADS, 1) backward_scan_kernel(Args a, int g
       clear(rh[e]);
       clear(rl[e]);
     }
-#pragma unroll 4
-    for (int ks = 0; ks < DK / 8; ++ks) {
-      float hi[4], lo[4];
-      get_split(gS, ks, lane, hi, lo);
+    if constexpr (B16) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        mma_apart<X>(rh[e], rl[e], hi, lo, pair(K + (own[e] * 8 + g) * L::PK + ks * 8 + 2 * t));
+      for (int kp = 0; kp < DK / 16; ++kp) {
+        const uint4 p[3] = {get_part(gS, kp, 0, lane), get_part(gS, kp, 1, lane), get_part(gS, kp, 2, lane)};
+        state_times<DK, L::PK, false>(rh, rl, p, K, kp, own, g, t);
+      }
+    } else {
+#pragma unroll 4
+      for (int ks = 0; ks < DK / 8; ++ks) {
+        float hi[4], lo[4];
+        get_split(gS, ks, lane, hi, lo);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          mma_apart<X>(rh[e], rl[e], hi, lo, pair(K + (own[e] * 8 + g) * L::PK + ks * 8 + 2 * t));
+      }
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -269,8 +281,13 @@ __global__ void __launch_bounds__(THREADS, 1) backward_scan_kernel(Args a, int g
         y[e][j] *= -f * ((j & 1) ? be.y : be.x);
         x[e][j] *= a.scale * f;
       }
-      put_split(gS, own[e], lane, y[e]);
-      put_split(gX, own[e], lane, x[e]);
+      if constexpr (B16) {
+        put_parts(gS, own[e], lane, y[e]);
+        put_parts(gX, own[e], lane, x[e]);
+      } else {
+        put_split(gS, own[e], lane, y[e]);
+        put_split(gX, own[e], lane, x[e]);
+      }
     }
     group_sync(grp);
 
@@ -280,18 +297,28 @@ __global__ void __launch_bounds__(THREADS, 1) backward_scan_kernel(Args a, int g
       clear(ah[n]);
       clear(al[n]);
     }
+    if constexpr (B16) {
 #pragma unroll
-    for (int ks = 0; ks < 8; ++ks) {
-      float hi[4], lo[4];
-      float2 kk[NT];
-      get_split(gS, ks, lane, hi, lo);
-      tiles_by_row<NT>(kk, K + ks * 8 * L::PK + kb, L::PK, lane);
+      for (int tp = 0; tp < 4; ++tp) {
+        const uint4 p[3] = {get_part(gS, tp, 0, lane), get_part(gS, tp, 1, lane), get_part(gS, tp, 2, lane)};
+        update_state<NT, L::PK>(ah, al, p, K + tp * 16 * L::PK + kb, lane);
+        const uint4 q[3] = {get_part(gX, tp, 0, lane), get_part(gX, tp, 1, lane), get_part(gX, tp, 2, lane)};
+        update_state<NT, L::PK>(ah, al, q, Q + tp * 16 * L::PK + kb, lane);
+      }
+    } else {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) mma_apart<X>(ah[n], al[n], hi, lo, kk[n]);
-      get_split(gX, ks, lane, hi, lo);
-      tiles_by_row<NT>(kk, Q + ks * 8 * L::PK + kb, L::PK, lane);
+      for (int ks = 0; ks < 8; ++ks) {
+        float hi[4], lo[4];
+        float2 kk[NT];
+        get_split(gS, ks, lane, hi, lo);
+        tiles_by_row<NT>(kk, K + ks * 8 * L::PK + kb, L::PK, lane);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) mma_apart<X>(ah[n], al[n], hi, lo, kk[n]);
+        for (int n = 0; n < NT; ++n) mma_apart<X>(ah[n], al[n], hi, lo, kk[n]);
+        get_split(gX, ks, lane, hi, lo);
+        tiles_by_row<NT>(kk, Q + ks * 8 * L::PK + kb, L::PK, lane);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_apart<X>(ah[n], al[n], hi, lo, kk[n]);
+      }
     }
     const float eC = eG[kC - 1];
 #pragma unroll

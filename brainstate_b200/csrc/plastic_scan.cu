@@ -172,7 +172,10 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(Args a, int groups, in
                 make_float2(s[n][2 * hf], s[n][2 * hf + 1]);
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n) put_split(gS, w * NT + n, lane, s[n]);
+    for (int n = 0; n < NT; ++n) {
+      if constexpr (SHORT) put_parts(gS, w * NT + n, lane, s[n]);
+      else put_split(gS, w * NT + n, lane, s[n]);
+    }
     group_sync(grp);
 
     // R^T and S^T Q^T of this warp's tokens
@@ -184,18 +187,23 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(Args a, int groups, in
       clear(zh[e]);
       clear(zl[e]);
     }
+    if constexpr (SHORT) {
 #pragma unroll
-    for (int ks = 0; ks < DK / 8; ++ks) {
-      float hi[4], lo[4];
-      get_split(gS, ks, lane, hi, lo);
+      for (int kp = 0; kp < DK / 16; ++kp) {
+        const uint4 x[3] = {get_part(gS, kp, 0, lane), get_part(gS, kp, 1, lane), get_part(gS, kp, 2, lane)};
+        state_times<DK, L::PK, false>(rh, rl, x, K, kp, own, g, t);
+        if (OUT) state_times<DK, L::PK, true>(zh, zl, x, Q, kp, own, g, t);
+      }
+    } else {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int at = (own[e] * 8 + g) * L::PK + ks * 8 + 2 * t;
-        mma_apart<X>(rh[e], rl[e], hi, lo, pair(K + at));
-        if (OUT) {
-          const float2 qq = pair(Q + at);
-          if (SHORT) mma(zh[e], hi, qq.x, qq.y);
-          else mma_apart<X>(zh[e], zl[e], hi, lo, qq);
+      for (int ks = 0; ks < DK / 8; ++ks) {
+        float hi[4], lo[4];
+        get_split(gS, ks, lane, hi, lo);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int at = (own[e] * 8 + g) * L::PK + ks * 8 + 2 * t;
+          mma_apart<X>(rh[e], rl[e], hi, lo, pair(K + at));
+          if (OUT) mma_apart<X>(zh[e], zl[e], hi, lo, pair(Q + at));
         }
       }
     }
@@ -234,7 +242,8 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(Args a, int groups, in
       u[e][1] *= ed.y;
       u[e][2] *= ed.x;
       u[e][3] *= ed.y;
-      put_split(gS, own[e], lane, u[e]);
+      if constexpr (SHORT) put_parts(gS, own[e], lane, u[e]);
+      else put_split(gS, own[e], lane, u[e]);
     }
     group_sync(grp);
 
@@ -245,14 +254,22 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(Args a, int groups, in
       clear(ah[n]);
       clear(al[n]);
     }
+    if constexpr (SHORT) {
 #pragma unroll
-    for (int ks = 0; ks < 8; ++ks) {
-      float hi[4], lo[4];
-      float2 kk[NT];
-      get_split(gS, ks, lane, hi, lo);
-      tiles_by_row<NT>(kk, K + ks * 8 * L::PK + kb, L::PK, lane);
+      for (int tp = 0; tp < 4; ++tp) {
+        const uint4 x[3] = {get_part(gS, tp, 0, lane), get_part(gS, tp, 1, lane), get_part(gS, tp, 2, lane)};
+        update_state<NT, L::PK>(ah, al, x, K + tp * 16 * L::PK + kb, lane);
+      }
+    } else {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) mma_apart<X>(ah[n], al[n], hi, lo, kk[n]);
+      for (int ks = 0; ks < 8; ++ks) {
+        float hi[4], lo[4];
+        float2 kk[NT];
+        get_split(gS, ks, lane, hi, lo);
+        tiles_by_row<NT>(kk, K + ks * 8 * L::PK + kb, L::PK, lane);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_apart<X>(ah[n], al[n], hi, lo, kk[n]);
+      }
     }
     const float eC = eG[kC - 1];
 #pragma unroll
@@ -265,7 +282,7 @@ __global__ void __launch_bounds__(THREADS, 1) scan_kernel(Args a, int groups, in
       for (int e = 0; e < 2; ++e) {
         const float2 eg = pair(eG + own[e] * 8 + 2 * t);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) zh[e][i] = a.scale * ((i & 1) ? eg.y : eg.x) * (SHORT ? zh[e][i] : zh[e][i] + zl[e][i]);
+        for (int i = 0; i < 4; ++i) zh[e][i] = a.scale * ((i & 1) ? eg.y : eg.x) * (zh[e][i] + zl[e][i]);
       }
       switch (w) {
         case 0: answer_own<0, SHORT>(gU, Pm, lane, zh); break;
