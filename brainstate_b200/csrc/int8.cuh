@@ -26,28 +26,29 @@ __device__ __forceinline__ E scaled(int sum, float sx, float sw) {
   return from_f<E>(__fmul_rn(__fmul_rn(mixed ? sw : s, sx), mixed ? s : sw));
 }
 
-// max|x| of a row or column as the ABI defines its scale: max / 127 in one rounding; NaN where an entry is not finite.
-__device__ __forceinline__ float scale_of(float top, bool finite) {
-  return finite ? __fdiv_rn(top, 127.f) : __int_as_float(0x7fffffff);
+// The scale of a row or column from its max|x| (max_nan): max / 127 in one rounding; NaN where an entry is not finite.
+__device__ __forceinline__ float scale_of(float top) {
+  return top <= 3.402823466e38f ? __fdiv_rn(top, 127.f) : __int_as_float(0x7fffffff);
 }
 
-// x / s to the nearest integer, ties to even, decided on the exact quotient: the 32-bit product x * (1/s) is within
-// 5e-5 of it, so only values that come within 1e-4 of a border need the 64-bit quotient.
+// x / s to the nearest integer, ties to even, decided on the exact quotient: the 32-bit product x * (1/s), |x/s| <= 127, is
+// within 127 * 2 * 2^-24 = 1.6e-5 of it (half of that without the product's own rounding), so only values that come as
+// near to a border need the 64-bit quotient.
 __device__ __forceinline__ int quantized(float x, float s, float inv) {
   const float y = x * inv;
   float n = rintf(y);
-  if (!(fabsf(y - n) < 0.4999f)) n = (float)rint((double)x / (double)s);
+  if (!(fabsf(y - n) < 0.49998f)) n = (float)rint((double)x / (double)s);
   return (int)fminf(fmaxf(n, -127.f), 127.f);
 }
 
 template <typename E> struct Stretch { E v[16 / sizeof(E)]; };
 
-__device__ __forceinline__ bool note(float x, float& top) {   // true for what is not finite
-  const float a = fabsf(x);
-  top = fmaxf(top, a);
-  return !(a <= 3.402823466e38f);
+// The larger of two, NaN if either is: a maximum of |x| that is finite says that all are.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
-
 // Four values in one word.  The nearest integer comes from the sum with 1.5 * 2^23, whose low byte is it; where a value
 // comes near a border the exact rule decides, out of line.
 static __device__ __noinline__ uint32_t four_exact(float4 x, float s, float inv) {
@@ -56,14 +57,36 @@ static __device__ __noinline__ uint32_t four_exact(float4 x, float s, float inv)
 }
 __device__ __forceinline__ uint32_t four(float4 x, float s, float inv) {
   constexpr float M = 12582912.f;
-  const float y0 = x.x * inv, y1 = x.y * inv, y2 = x.z * inv, y3 = x.w * inv;
-  const float t0 = __fadd_rn(y0, M), t1 = __fadd_rn(y1, M), t2 = __fadd_rn(y2, M), t3 = __fadd_rn(y3, M);
-  const float d = fmaxf(fmaxf(fabsf(y0 - __fsub_rn(t0, M)), fabsf(y1 - __fsub_rn(t1, M))),
-                        fmaxf(fabsf(y2 - __fsub_rn(t2, M)), fabsf(y3 - __fsub_rn(t3, M))));
-  if (!(d < 0.4999f)) return four_exact(x, s, inv);
+  const float t0 = fmaf(x.x, inv, M), t1 = fmaf(x.y, inv, M), t2 = fmaf(x.z, inv, M), t3 = fmaf(x.w, inv, M);
+  const float d = fmaxf(fmaxf(fabsf(fmaf(x.x, inv, M - t0)), fabsf(fmaf(x.y, inv, M - t1))),
+                        fmaxf(fabsf(fmaf(x.z, inv, M - t2)), fabsf(fmaf(x.w, inv, M - t3))));
+  if (!(d < 0.49999f)) return four_exact(x, s, inv);
   return __byte_perm(__byte_perm(__float_as_uint(t0), __float_as_uint(t1), 0x0040),
                      __byte_perm(__float_as_uint(t2), __float_as_uint(t3), 0x0040), 0x5410);
 }
+
+// The running max|x| of 16-byte stretches: two 16-bit entries an instruction.
+template <typename X> struct Top {
+  float t = 0.f;
+  __device__ __forceinline__ void look(const int4& w) {
+    const Stretch<X> h = *reinterpret_cast<const Stretch<X>*>(&w);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t = max_nan(t, fabsf(h.v[e]));
+  }
+  __device__ __forceinline__ float get() const { return t; }
+};
+template <typename X2, typename X> struct Top2 {
+  X2 t;
+  __device__ __forceinline__ Top2() { *reinterpret_cast<uint32_t*>(&t) = 0u; }
+  __device__ __forceinline__ void look(const int4& w) {
+    const X2* h = reinterpret_cast<const X2*>(&w);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t = __hmax2_nan(t, __habs2(h[e]));
+  }
+  __device__ __forceinline__ float get() const { return max_nan(to_f<X>(t.x), to_f<X>(t.y)); }
+};
+template <> struct Top<__nv_bfloat16> : Top2<__nv_bfloat162, __nv_bfloat16> {};
+template <> struct Top<__half> : Top2<__half2, __half> {};
 
 // Rows of a product's left operand are padded to whole 16-byte stretches.
 inline int64_t padded(int64_t k) { return (k + 15) / 16 * 16; }

@@ -48,35 +48,30 @@ __device__ __forceinline__ void take_rows(const void* x, int64_t stride, int M, 
     const X* xr = static_cast<const X*>(x) + row * stride;
     const int4* x4 = reinterpret_cast<const int4*>(xr);
     float top = 0.f;
-    bool bad = false;
     const int n = on ? K / V : 0;
     int4 held[2];      // the first two stretches stay in registers between the passes
     if (vec) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) held[i] = at + i * T < n ? __ldg(x4 + at + i * T) : make_int4(0, 0, 0, 0);
       ask_weights();
-      auto look = [&](const int4& w) {
-        const Stretch<X> h = *reinterpret_cast<const Stretch<X>*>(&w);
-#pragma unroll
-        for (int e = 0; e < V; ++e) bad |= note(to_f<X>(h.v[e]), top);
-      };
-      look(held[0]);
-      look(held[1]);
+      Top<X> look;
+      look.look(held[0]);
+      look.look(held[1]);
 #pragma unroll 4
-      for (int c = at + 2 * T; c < n; c += T) look(__ldg(x4 + c));
+      for (int c = at + 2 * T; c < n; c += T) look.look(__ldg(x4 + c));
+      top = look.get();
     } else {
       ask_weights();
-      for (int c = at; on && c < K; c += T) bad |= note(to_f<X>(xr[c]), top);
+      for (int c = at; on && c < K; c += T) top = max_nan(top, fabsf(to_f<X>(xr[c])));
     }
-    if (bad) top = __int_as_float(0x7f800000);     // finite maxima stay below
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (lane == 0) part[warp] = top;
     __syncthreads();
     top = part[row * WPR];
 #pragma unroll
-    for (int w = 1; w < WPR; ++w) top = fmaxf(top, part[row * WPR + w]);
-    const float s = scale_of(top, top <= 3.402823466e38f);
+    for (int w = 1; w < WPR; ++w) top = max_nan(top, part[row * WPR + w]);
+    const float s = scale_of(top);
     if (at == 0) scale[row] = s;
     const bool zero = !(s > 0.f);
     const float inv = s < 1e-30f ? __int_as_float(0x7fffffff) : 1.f / s;

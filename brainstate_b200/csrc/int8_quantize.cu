@@ -7,7 +7,7 @@
 namespace bsx {
 namespace int8 {
 
-constexpr int kHeld = 2;   // 16-byte stretches a thread keeps between the two passes over its row
+constexpr int kHeld = 4;   // 16-byte stretches a thread keeps between the two passes over its row
 
 // One block per row: the maximum, then the values.  Bound by reading the row once and writing a byte per entry; the first
 // kHeld 16-byte stretches of a thread stay in registers in between, the rest comes from L2 the second time.
@@ -22,46 +22,35 @@ quantize_rows_kernel(const E* __restrict__ x, int64_t stride, int64_t K, int64_t
   const E* xr = x + row * stride;
   int8_t* qr = q + row * Kp;
   let_dependents_start();
-  Stretch<E> held[kHeld];
+  int4 held[kHeld];
   float top = 0.f;
-  bool bad = false;
   const int n = (int)(K / V);
   const int4* x4 = reinterpret_cast<const int4*>(xr);
   if (VEC) {
+    Top<E> look;
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i)
-      if (tid + i * THREADS < n) {
-        const int4 w = __ldg(x4 + tid + i * THREADS);
-        held[i] = *reinterpret_cast<const Stretch<E>*>(&w);
-      }
+    for (int i = 0; i < kHeld; ++i) held[i] = tid + i * THREADS < n ? __ldg(x4 + tid + i * THREADS) : make_int4(0, 0, 0, 0);
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i)
-      if (tid + i * THREADS < n) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) bad |= note(to_f<E>(held[i].v[e]), top);
-      }
-    for (int c = tid + kHeld * THREADS; c < n; c += THREADS) {
-      const int4 w = __ldg(x4 + c);
-      const Stretch<E> h = *reinterpret_cast<const Stretch<E>*>(&w);
-#pragma unroll
-      for (int e = 0; e < V; ++e) bad |= note(to_f<E>(h.v[e]), top);
-    }
+    for (int i = 0; i < kHeld; ++i) look.look(held[i]);
+    for (int c = tid + kHeld * THREADS; c < n; c += THREADS) look.look(__ldg(x4 + c));
+    top = look.get();
   } else {
-    for (int c = tid; c < K; c += THREADS) bad |= note(to_f<E>(xr[c]), top);
+    for (int c = tid; c < K; c += THREADS) top = max_nan(top, fabsf(to_f<E>(xr[c])));
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (lane == 0) part[tid >> 5] = top;
-  const bool finite = !__syncthreads_or(bad);
+  __syncthreads();
   top = part[lane % (THREADS / 32)];
 #pragma unroll
-  for (int o = THREADS / 64; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float s = scale_of(top, finite);
+  for (int o = THREADS / 64; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float s = scale_of(top);
   if (tid == 0) scale[row] = s;
-  const bool zero = !finite || s == 0.f;
+  const bool zero = !(s > 0.f);
   const float inv = s < 1e-30f ? __int_as_float(0x7fffffff) : 1.f / s;   // tiny scales: every quotient in 64 bits
   if (VEC) {
-    auto put = [&](int c, const Stretch<E>& h) {
+    auto put = [&](int c, const int4& x) {
+      const Stretch<E> h = *reinterpret_cast<const Stretch<E>*>(&x);
       uint32_t w[V / 4];
 #pragma unroll
       for (int e = 0; e < V; e += 4)
@@ -73,10 +62,7 @@ quantize_rows_kernel(const E* __restrict__ x, int64_t stride, int64_t K, int64_t
 #pragma unroll
     for (int i = 0; i < kHeld; ++i)
       if (tid + i * THREADS < n) put(tid + i * THREADS, held[i]);
-    for (int c = tid + kHeld * THREADS; c < n; c += THREADS) {
-      const int4 w = __ldg(x4 + c);
-      put(c, *reinterpret_cast<const Stretch<E>*>(&w));
-    }
+    for (int c = tid + kHeld * THREADS; c < n; c += THREADS) put(c, __ldg(x4 + c));
     for (int c = n + tid; c < (int)(Kp / V); c += THREADS) {
       if (V == 8) reinterpret_cast<uint2*>(qr)[c] = make_uint2(0u, 0u);
       else reinterpret_cast<uint32_t*>(qr)[c] = 0u;
@@ -127,11 +113,10 @@ __global__ void __launch_bounds__(256) column_top_kernel(const E* __restrict__ w
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t n = (int64_t)blockIdx.x * 32 + tx;
   float t = 0.f;
-  bool bad = false;
   if (n < N)
 #pragma unroll 4
-    for (int64_t k = (int64_t)blockIdx.y * 8 + ty; k < K; k += (int64_t)gridDim.y * 8) bad |= note(to_f<E>(w[k * N + n]), t);
-  part[ty][tx] = bad ? __int_as_float(0x7f800000) : t;
+    for (int64_t k = (int64_t)blockIdx.y * 8 + ty; k < K; k += (int64_t)gridDim.y * 8) t = max_nan(t, fabsf(to_f<E>(w[k * N + n])));
+  part[ty][tx] = t <= 3.402823466e38f ? t : __int_as_float(0x7f800000);
   __syncthreads();
   if (ty == 0 && n < N) {
 #pragma unroll
@@ -149,7 +134,7 @@ quantize_columns_kernel(const E* __restrict__ w, int64_t K, int64_t N, int64_t K
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t n0 = (int64_t)blockIdx.x * 32, n = n0 + tx, k0 = (int64_t)blockIdx.y * 128;
   const float t = n < N ? __uint_as_float(top[n]) : 0.f;
-  const float s = scale_of(t, t <= 3.402823466e38f);
+  const float s = scale_of(t);
   const bool zero = !(s > 0.f);
   const float inv = s < 1e-30f ? __int_as_float(0x7fffffff) : 1.f / s;
 #pragma unroll 4
@@ -169,7 +154,7 @@ quantize_columns_kernel(const E* __restrict__ w, int64_t K, int64_t N, int64_t K
 // ... and the maxima become scales.
 __global__ void __launch_bounds__(256) column_scale_kernel(float* scale, int64_t N) {
   const int64_t n = blockIdx.x * 256ll + threadIdx.x;
-  if (n < N) scale[n] = scale_of(scale[n], scale[n] <= 3.402823466e38f);
+  if (n < N) scale[n] = scale_of(scale[n]);
 }
 
 template <typename E>
@@ -192,10 +177,10 @@ template <typename E, bool VEC>
 static void launch_rows_vec(const E* x, int64_t stride, int64_t M, int64_t K, int8_t* q, float* scale, cudaStream_t st) {
   const int64_t Kp = padded(K);
   // few rows: the time is that of one row, so that as many threads as its stretches fill share it
-  if (M < 148 && K * (int64_t)sizeof(E) > 256 * 16)
+  if (M < 148 && K * (int64_t)sizeof(E) > 128 * 16)
     quantize_rows_kernel<E, VEC, 1024><<<(unsigned)M, 1024, 0, st>>>(x, stride, K, Kp, q, scale);
   else
-    quantize_rows_kernel<E, VEC, 256><<<(unsigned)M, 256, 0, st>>>(x, stride, K, Kp, q, scale);
+    quantize_rows_kernel<E, VEC, 128><<<(unsigned)M, 128, 0, st>>>(x, stride, K, Kp, q, scale);
 }
 
 template <typename E>

@@ -258,20 +258,38 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
   }
 }
 
-// Adds the partial sums of a split inner dimension and scales.
-template <typename E>
+// Adds the partial sums of a split inner dimension and scales: four channels a thread, a block 1024 of a row.
+template <typename E, bool VEC>
 __global__ void __launch_bounds__(256) add_splits_kernel(Product p, int splits) {
-  const int64_t total = p.M * p.N;
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    int s = 0;
+  const int64_t n = (int64_t)blockIdx.x * 1024 + threadIdx.x * 4;
+  if (n >= p.N) return;
+  float sw[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sw[j] = n + j < p.N ? __ldg(p.sw + n + j) : 0.f;
+  for (int64_t m = blockIdx.y; m < p.M; m += gridDim.y) {
+    const int32_t* x = p.partial + m * p.N + n;
+    int s[4] = {0, 0, 0, 0};
     bool whole = true;
-    for (int k = 0; k < splits; ++k) {
-      const int x = __ldg(p.partial + k * total + i);
-      whole &= x != kNoSum;
-      s += x;
+    for (int k = 0; k < splits; ++k, x += p.M * p.N) {
+      int v[4];
+      if (VEC) {
+        const int4 q = __ldg(reinterpret_cast<const int4*>(x));
+        v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = n + j < p.N ? __ldg(x + j) : 0;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        whole &= v[j] != kNoSum;
+        s[j] += v[j];
+      }
     }
-    const int64_t m = i / p.N, n = i - m * p.N;
-    static_cast<E*>(p.out)[i] = scaled<E>(s, whole ? __ldg(p.sx + m) : __int_as_float(0x7fffffff), __ldg(p.sw + n));
+    const float sx = whole ? __ldg(p.sx + m) : __int_as_float(0x7fffffff);
+    E* o = static_cast<E*>(p.out) + m * p.N + n;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (n + j < p.N) o[j] = scaled<E>(s[j], sx, sw[j]);
   }
 }
 
@@ -280,7 +298,7 @@ static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // How a product is divided: rows of a tile and splits of the inner dimension, the cheapest by an estimate in clocks.
 // Measured on a B200: a step of 128 takes 776 clocks with 256 rows and 653 with 128 (about 284 and 0.015 a byte that a
 // block copies, whose rate from L2 is the limit; the instructions alone would take 512 and 256); a tile's output about
-// 1000 and 20 a row; adding splits costs a launch (6500) and its bytes (4400 a clock over the card).
+// 1000 and 20 a row; adding splits costs a launch and its latency (7000) and its bytes (3000 a clock over the card).
 Plan plan_tiles(int64_t M, int64_t N, int64_t Kp, int sms) {
   const int64_t pairs = sms > 1 ? sms / 2 : 74, steps = ceil_div(Kp, kBK);
   Plan best = {32, 1};
@@ -290,7 +308,7 @@ Plan plan_tiles(int64_t M, int64_t N, int64_t Kp, int sms) {
     for (int s = 1; s <= 8 && s <= steps; s *= 2) {
       const int64_t waves = ceil_div(ceil_div(N, 2 * kBM) * ceil_div(M, bt) * s, pairs);
       double cost = waves * ceil_div(steps, s) * step + out;
-      if (s > 1) cost += 6500 + (double)M * N * s * 8 / 4400;
+      if (s > 1) cost += 7000 + (double)M * N * s * 8 / 3000;
       if (least == 0 || cost < least) {
         least = cost;
         best = {bt, s};
@@ -348,8 +366,9 @@ static int launch_height(const Product& p, int splits, int sms, cudaStream_t st)
                                       Tiles<BT>::bytes, st, mw, mx, p, w);
   if (e != cudaSuccess) return cuda_fail(e, "int8 tiles_kernel");
   if (SPLIT) {
-    const int64_t want = ceil_div(p.M * p.N, 256), most = 8ll * sms;
-    add_splits_kernel<E><<<(unsigned)(want < most ? want : most), 256, 0, st>>>(p, splits);
+    const dim3 grid((unsigned)ceil_div(p.N, 1024), (unsigned)(p.M < 65535 ? p.M : 65535));
+    if (p.N % 4 == 0 && aligned16(p.partial)) add_splits_kernel<E, true><<<grid, 256, 0, st>>>(p, splits);
+    else add_splits_kernel<E, false><<<grid, 256, 0, st>>>(p, splits);
     BSX_LAUNCH_CHECK("int8 add_splits_kernel");
   }
   return BSX_OK;
