@@ -11,6 +11,10 @@
 // tensor memory.  Pairs take tiles in a fixed stride; for few tiles and a long inner dimension several pairs share a
 // tile's inner dimension, write their integer sums to the workspace, and a second kernel adds them.
 //
+// 4096 x 4096 by 4096 x 8192: 122 us, 2.25e15 operations a second (69 % of twice the measured bf16 rate), the tensor unit 56 %
+// busy: 32 KB a block and step come from L2 at 43 bytes a clock and SM, 12 TB/s over the card, in 775 clocks where the
+// instructions take 512.  Blocks of their own (128 x 256) read half as much again and took 125 us.
+//
 // Every wait is bounded.  A block whose wait runs out waits (again with a bound) for its copies in flight, takes no more
 // part and leaves NaN in its tiles.
 #include <cuda.h>

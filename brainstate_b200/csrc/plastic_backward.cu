@@ -5,7 +5,8 @@
 // operands).  With dS the cotangent of the state after the chunk:
 //   dU = P^T dO + diag(e^{G_C-G}) K dS,  dY = T^T dU,  dV = beta dY,  dR = -beta e^G dY,
 //   dS <- e^{G_C} dS + Q^T (scale e^G dO) + K^T dR.
-// It leaves dS (before the update) and dY for every chunk.
+// It leaves dS (before the update) and dY for every chunk.  4 x 2048 tokens of 16 heads of 128 x 128 in bf16: 259 us, bound
+// like the forward pass (shared memory 53 %, tensor unit 41 %).
 //
 // backward_chunk_kernel: everything else, independent of the order of the chunks; each block of 16 warps takes one (row, head,
 // chunk) after the other and copies the next one's data while it finishes one.  Over blocks of 32 value columns it
@@ -15,6 +16,8 @@
 //   dbeta_i = dY_i.V_i - e^{G_i} K_i.D1_i + sum_j dA_ij (A/beta)_ij
 //   dG_i = -beta e^G K_i.D1_i + scale e^G Q_i.Dq_i - e^{G_C-G} K_i.D3_i + (row - column sums of dP P + dA A)_i,
 //   dG_C += sum_i e^{G_C-G_i} K_i.D3_i + e^{G_C} <S0, dS>,   dg = sums of dG from the chunk's end.
+// The same sizes: 464 us (tensor unit 40 %, issue slots 47 %).  Its 128 registers a thread hold the sums of all five
+// products, which is what bounds the tiles; eight warps with twice the registers took 820 us.
 #include <type_traits>
 
 #include "plastic.cuh"

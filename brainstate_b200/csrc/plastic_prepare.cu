@@ -7,6 +7,9 @@
 // T_ij = -sum_l (T_ii A_il) T_lj, warp i having block row i, on split operands.  (A power series would need fewer steps but
 // loses all digits when the keys of a chunk are alike.)  The sums of g are taken in 64 bits and kept as two floats, so
 // that a strong decay (g is cut at -128, where e^g is 0 in 32 bits) leaves the differences behind it exact.
+//
+// A chain of short phases (no pipe above 54 %), four blocks to an SM: 2048 chunks of dk = 128 in bf16 take 53 us, of which
+// reading the tiles and writing them, T and P would take 31 us.
 #include "plastic.cuh"
 
 namespace bsx {

@@ -235,5 +235,6 @@ def delta_rule_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.
     d = _DESC.pack(B, 1, Hk, Hv, dk, dv, _TYPES[q.dtype], dk ** -0.5 if scale is None else scale, q.data_ptr(), k.data_ptr(),
                    v.data_ptr(), g.data_ptr(), beta.data_ptr(), at, 0, qb, 0, qh, kb, 0, kh, vb, 0, vh, gb, 0, gh, bb, 0, bh)
     call_on(v.get_device(), lib().bsx_delta_recurrent, d, o.data_ptr(), at)
-    torch.autograd.graph.increment_version(state)
+    if not state.is_inference():       # such tensors have no version: nothing was recorded with them
+        torch.autograd.graph.increment_version(state)
     return o

@@ -374,6 +374,26 @@ def test_saved_state_is_guarded(cuda):
         o.sum().backward()
 
 
+def test_inference_mode(cuda):
+    """Serving: states made inside and outside of inference mode."""
+    from brainstate_b200 import nn, plastic
+    args = {n: x.cuda() for n, x in inputs(2, 20, 1, 2, 16, 16, F32).items()}
+    initial = args.pop('initial')
+    want, state = plastic.delta_rule(*args.values(), initial_state=initial)
+    outside = initial.clone()
+    with torch.inference_mode():
+        o, s = plastic.delta_rule(*args.values(), initial_state=initial)
+        assert torch.equal(o, want) and torch.equal(s, state)
+        inside = initial.clone()
+        for st in (inside, outside):
+            y = plastic.delta_rule_step(*(x[:, 0] for x in args.values()), st)
+            assert error(y, want[:, 0].cpu()) <= 1e-5
+        assert torch.equal(inside, outside)
+        layer = nn.DeltaSynapse(16, 16, v_heads=2)
+        layer.init_state(2)
+        layer(*(x[:, 0] for x in args.values()))
+
+
 def test_refusals_on_device_tensors(cuda):
     from brainstate_b200 import plastic
     a = {n: x.cuda() for n, x in inputs(2, 20, 2, 4, 8, 8, F32).items()}

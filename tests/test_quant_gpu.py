@@ -59,6 +59,8 @@ def test_product(cuda, dtype, M, K, N):
     assert y.dtype == dtype
     close(y, want, dtype)
     assert torch.equal(rows @ w8, y)
+    assert torch.equal(rows.dequantize().cpu(), (xq * xs.unsqueeze(1)).float())
+    assert torch.equal(w8.dequantize().cpu(), (wq * ws.unsqueeze(1)).float().t())
     close(quant.int8_matmul(x.cuda(), w8, out_dtype=F32), want, F32)
 
 
