@@ -131,7 +131,7 @@ template <typename E>
 __global__ void __launch_bounds__(256)
 quantize_columns_kernel(const E* __restrict__ w, int64_t K, int64_t N, int64_t Kp, int8_t* __restrict__ q,
                         const uint32_t* __restrict__ top) {
-  __shared__ int8_t tile[32][132];
+  __shared__ __align__(16) int8_t tile[32][132];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t n0 = (int64_t)blockIdx.x * 32, n = n0 + tx, k0 = (int64_t)blockIdx.y * 128;
   const float t = n < N ? __uint_as_float(top[n]) : 0.f;

@@ -237,7 +237,8 @@ def test_gradients_against_differences(cuda):
 
 @pytest.mark.parametrize('dtype', [F32, BF16, F16])
 @pytest.mark.parametrize('B,Hk,Hv,dk,dv', [(1, 1, 1, 1, 1), (3, 2, 4, 33, 20), (2, 2, 2, 64, 64), (5, 1, 3, 128, 132),
-                                           (70, 2, 4, 128, 128)])
+                                           (70, 2, 4, 128, 128), (400, 2, 4, 128, 128), (601, 1, 2, 64, 36),
+                                           (310, 2, 4, 113, 128), (300, 1, 4, 128, 112), (1200, 1, 1, 16, 16)])
 def test_steps_in_place(cuda, dtype, B, Hk, Hv, dk, dv):
     """Several single steps: each output and the last state against the definition, and the state tensor is the same."""
     from brainstate_b200 import plastic
