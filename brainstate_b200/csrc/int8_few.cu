@@ -207,7 +207,7 @@ int launch_few(const Product& p, int dtype, cudaStream_t st) {
 
 // Every block reads and quantises all rows: M / 8 of the weights' traffic (for 16-bit rows), from L2, and M * K / 512 values a
 // thread.  One row of 8192 x 4096: 9.1 us replayed in a graph against 7.8 us with a kernel of its own for the rows, but
-// 12.5 us against 18.7 us of host time where calls are launched one by one; 1000 x 2000 3.5 us against 3.8 us.
+// 11.1 us against 15.3 us of host time where calls are launched one by one; 1000 x 2000 3.5 us against 3.8 us.
 bool few_takes_rows(int64_t M, int64_t K) { return M <= 4 && M * padded(K) <= 40704; }
 
 template <typename E, typename X, int EVENT>

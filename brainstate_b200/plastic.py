@@ -40,23 +40,29 @@ RECURRENT_TOKENS = 8
 
 
 def _dense_rows(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+    return t if t.stride(-1) == 1 else t.contiguous()      # contiguous() leaves a dimension of one entry as it is
+
+
+def _dense_like(t: torch.Tensor) -> torch.Tensor:
+    """A new dense tensor of this shape and type.  From a dense tensor in two thirds of the host's time for a shape."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
 
 
 def _describe(q, k, v, g, beta, initial, lengths, scale) -> bytes:
     B, T, Hk, dk = q.shape
-    Hv, dv = v.shape[2:]
+    _, _, Hv, dv = v.shape
+    (qb, qt, qh, _), (kb, kt, kh, _), (vb, vt, vh, _) = q.stride(), k.stride(), v.stride()
     return _DESC.pack(B, T, Hk, Hv, dk, dv, _TYPES[q.dtype], scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
                       beta.data_ptr(), 0 if initial is None else initial.data_ptr(),
-                      0 if lengths is None else lengths.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+                      0 if lengths is None else lengths.data_ptr(), qb, qt, qh, kb, kt, kh, vb, vt, vh,
                       *g.stride(), *beta.stride())
 
 
 def _forward(q, k, v, g, beta, initial, lengths, scale):
     B, T, _, dk = q.shape
-    Hv, dv = v.shape[2:]
-    o = v.new_empty((B, T, Hv, dv))
-    state = g.new_empty((B, Hv, dk, dv))
+    _, _, Hv, dv = v.shape
+    o = _dense_like(v)
+    state = g.new_empty((B, Hv, dk, dv)) if initial is None else _dense_like(initial)
     d = _describe(q, k, v, g, beta, initial, lengths, scale)
     if T <= RECURRENT_TOKENS:
         call_on(v.get_device(), lib().bsx_delta_recurrent, d, o.data_ptr(), state.data_ptr())
@@ -83,10 +89,10 @@ class _DeltaRule(torch.autograd.Function):
             return (None,) * 8
         q, k, v, g, beta, initial, lengths = ctx.saved_tensors
         # dense whatever the strides of the inputs
-        dq, dk, dv, dg, dbeta = (t.new_empty(t.shape) for t in (q, k, v, g, beta))
+        dq, dk, dv, dg, dbeta = _dense_like(q), _dense_like(k), _dense_like(v), _dense_like(g), _dense_like(beta)
         do = v.new_zeros(v.shape) if do is None else do.contiguous()
         dstate = None if dstate is None else dstate.contiguous()
-        dinitial = initial.new_empty(initial.shape) if ctx.needs_input_grad[5] else None
+        dinitial = _dense_like(initial) if ctx.needs_input_grad[5] else None
         d = _describe(q, k, v, g, beta, initial, lengths, ctx.scale)
         n = lib().bsx_delta_backward_workspace_bytes(d)
         ws = g.new_empty(n // 4)
@@ -107,7 +113,7 @@ def _fits(q, k, v, g, beta, state, lead: int) -> bool:
                 and qs[lead] > 0 and vs[lead] > 0 and vs[lead] % qs[lead] == 0 and 1 <= qs[-1] <= 128
                 and 1 <= vs[-1] <= 4096
                 and (state is None or (state.dtype == torch.float32 and state.get_device() == dev
-                                       and tuple(state.shape) == (qs[0], vs[lead], qs[-1], vs[-1]))))
+                                       and state.shape == (qs[0], vs[lead], qs[-1], vs[-1]))))
     except AttributeError:
         return False
 
@@ -202,7 +208,8 @@ def delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
         initial_state = initial_state.contiguous()
     args = (_dense_rows(q), _dense_rows(k), _dense_rows(v), g, beta, initial_state, lengths,
             q.shape[-1] ** -0.5 if scale is None else float(scale))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:6]):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad
+                                    or beta.requires_grad or (initial_state is not None and initial_state.requires_grad)):
         return _DeltaRule.apply(*args)
     return _forward(*args)
 
@@ -220,17 +227,21 @@ def delta_rule_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.
     _check(q, k, v, g, beta, state, 1)
     if not state.is_contiguous():
         raise ValueError('the state must be contiguous: it is updated in place')
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, g, beta, state)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad
+                                    or beta.requires_grad or state.requires_grad):
         raise RuntimeError('delta_rule_step updates the state in place and records no gradient: '
                            'use delta_rule, or call it under torch.no_grad()')
-    q, k, v = _dense_rows(q), _dense_rows(k), _dense_rows(v)
+    (qb, qh, qc), (kb, kh, kc), (vb, vh, vc) = q.stride(), k.stride(), v.stride()
+    if qc != 1 or kc != 1 or vc != 1:
+        q, k, v = _dense_rows(q), _dense_rows(k), _dense_rows(v)
+        (qb, qh, _), (kb, kh, _), (vb, vh, _) = q.stride(), k.stride(), v.stride()
     if g.dtype != torch.float32:
         g = g.to(torch.float32)
     if beta.dtype != torch.float32:
         beta = beta.to(torch.float32)
     (B, Hk, dk), (_, Hv, dv) = q.shape, v.shape
-    o = v.new_empty((B, Hv, dv))
-    (qb, qh, _), (kb, kh, _), (vb, vh, _), (gb, gh), (bb, bh) = q.stride(), k.stride(), v.stride(), g.stride(), beta.stride()
+    o = _dense_like(v)
+    (gb, gh), (bb, bh) = g.stride(), beta.stride()
     at = state.data_ptr()
     d = _DESC.pack(B, 1, Hk, Hv, dk, dv, _TYPES[q.dtype], dk ** -0.5 if scale is None else scale, q.data_ptr(), k.data_ptr(),
                    v.data_ptr(), g.data_ptr(), beta.data_ptr(), at, 0, qb, 0, qh, kb, 0, kh, vb, 0, vh, gb, 0, gh, bb, 0, bh)

@@ -10,6 +10,7 @@ There is no gradient: train in float (``EventLinear``), then quantise.
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -21,7 +22,14 @@ from .event import EventArray, _require_cuda
 __all__ = ['Int8Dense', 'Int8Rows', 'quantize_rows', 'int8_matmul']
 
 _TYPES = {torch.float32: _lib.T_F32, torch.bfloat16: _lib.T_BF16, torch.float16: _lib.T_F16}
+_MATMULS = (torch.Tensor.__matmul__, torch.Tensor.matmul, torch.matmul)
 _EVENTS = {torch.bool: _lib.T_EVENT8, torch.uint8: _lib.T_EVENT8, torch.float32: _lib.T_EVENT32}
+
+
+@lru_cache(maxsize=4096)
+def _workspace_bytes(given: bool, m: int, n_pre: int, n_post: int) -> int:
+    """Workspace of a product over ``given`` 8-bit rows, or of one that quantises them."""
+    return (lib().bsx_int8_matmul_workspace_bytes if given else lib().bsx_int8_dense_workspace_bytes)(m, n_pre, n_post)
 
 
 def _rows(x, n: Optional[int]):
@@ -116,8 +124,7 @@ class Int8Dense:
     @classmethod
     def __torch_function__(cls, func, types, args=(), kwargs=None):
         # ``tensor @ w`` comes here first; sent on, it would reach __rmatmul__ only after an error was raised and dropped
-        if func in (torch.Tensor.__matmul__, torch.Tensor.matmul, torch.matmul) and not kwargs and len(args) == 2 \
-                and isinstance(args[1], cls):
+        if func in _MATMULS and not kwargs and len(args) == 2 and isinstance(args[1], cls):
             return int8_matmul(*args)
         return NotImplemented
 
@@ -144,14 +151,14 @@ def int8_matmul(x, w: Int8Dense, out_dtype: Optional[torch.dtype] = None) -> tor
     m, dev = data.shape[0], data.get_device()
     if dev != w.q.get_device():
         raise ValueError(f'input is on {data.device}, the weights on {w.q.device}')
-    out = data.new_empty(lead + (n_post,), dtype=kind)
+    out = data.new_empty(lead + (n_post,)) if kind is data.dtype else data.new_empty(lead + (n_post,), dtype=kind)
     if rows:
-        n = lib().bsx_int8_matmul_workspace_bytes(m, n_pre, n_post)
+        n = _workspace_bytes(True, m, n_pre, n_post)
         ws = data.new_empty(n) if n else None
         call_on(dev, lib().bsx_int8_matmul, data.data_ptr(), x.scale.data_ptr(), w.q.data_ptr(), w.scale.data_ptr(), m, n_pre,
                 n_post, out.data_ptr(), _TYPES[kind], None if ws is None else ws.data_ptr(), n)
     else:
-        n = lib().bsx_int8_dense_workspace_bytes(m, n_pre, n_post)
+        n = _workspace_bytes(False, m, n_pre, n_post)
         ws = w.q.new_empty(n) if n else None
         call_on(dev, lib().bsx_int8_dense, data.data_ptr(), fmt, data.stride(0), w.q.data_ptr(), w.scale.data_ptr(), m, n_pre,
                 n_post, out.data_ptr(), _TYPES[kind], None if ws is None else ws.data_ptr(), n)
