@@ -8,8 +8,9 @@
 // loses all digits when the keys of a chunk are alike.)  The sums of g are taken in 64 bits and kept as two floats, so
 // that a strong decay (g is cut at -128, where e^g is 0 in 32 bits) leaves the differences behind it exact.
 //
-// A chain of short phases (no pipe above 54 %), four blocks to an SM: 2048 chunks of dk = 128 in bf16 take 53 us, of which
-// reading the tiles and writing them, T and P would take 31 us.
+// A chain of short phases whose waits blocks hide for each other, six to an SM (T and A lie where K and Q were; with four
+// it took 52 us): 2048 chunks of dk = 128 in bf16 take 46 us, of which reading the tiles and writing them, T and P would
+// take 31 us.
 #include "plastic.cuh"
 
 namespace bsx {
@@ -20,9 +21,28 @@ struct PrepLayout {
   static constexpr int PK = DK + 8;  // pair loads of 8 rows hit distinct banks
   static constexpr size_t tile = (size_t)kC * PK * sizeof(E);
   static constexpr int PA = kC + 4;  // as right operand rows 2t, 2t + 1 hit distinct banks
-  static_assert(2 * tile >= sizeof(float) * kC * PA, "T takes the place of the K and Q tiles");
-  static constexpr size_t bytes = 2 * tile + sizeof(float) * (kC * PA + 3 * kC);
+  // T and A take the place of the K and Q tiles
+  static constexpr size_t matrix = sizeof(float) * kC * PA, shared = tile > matrix ? 2 * tile : 2 * matrix;
+  static constexpr size_t bytes = shared + sizeof(float) * 3 * kC;
 };
+
+// 16 x 8 x 16 with 16-bit operands: their products are exact in the float32 sums.
+template <typename E>
+__device__ __forceinline__ void mma_exact(float* c, const uint4& a, uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<E, __nv_bfloat16>::value)
+    mma16(c, a, b0, b1);
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+// A left operand: four 8 x 8 tiles, a row's address from each lane.
+__device__ __forceinline__ uint4 four_tiles(const void* row) {
+  uint4 r;
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(smem_u32(row)) : "memory");
+  return r;
+}
 
 template <typename E, int DK, bool BACK>
 __global__ void __launch_bounds__(128) prepare_kernel(Args a) {
@@ -30,9 +50,9 @@ __global__ void __launch_bounds__(128) prepare_kernel(Args a) {
   extern __shared__ __align__(16) unsigned char smem[];
   E* sk = reinterpret_cast<E*>(smem);
   E* sq = reinterpret_cast<E*>(smem + L::tile);
-  float* sA = reinterpret_cast<float*>(smem + 2 * L::tile);
   float* sT = reinterpret_cast<float*>(smem);      // once K and Q are not needed any more
-  float* sHi = sA + kC * L::PA;
+  float* sA = reinterpret_cast<float*>(smem + L::matrix);
+  float* sHi = reinterpret_cast<float*>(smem + L::shared);
   float* sLo = sHi + kC;
   float* sBeta = sLo + kC;
 
@@ -106,19 +126,28 @@ __global__ void __launch_bounds__(128) prepare_kernel(Args a) {
     clear(kk[u]);
     clear(qk[u]);
   }
+  if constexpr (IsExact<E>::value) {
 #pragma unroll 2
-  for (int ks = 0; ks < DK / 8; ++ks) {
-    const int c = ks * 8 + 2 * t;
+    for (int kp = 0; kp < DK / 16; ++kp)
 #pragma unroll
-    for (int u = 0; u < 5; ++u) {
-      const float2 k0 = pair(sk + r0[u] * L::PK + c), k1 = pair(sk + (r0[u] + 8) * L::PK + c);
-      const float2 q0 = pair(sq + r0[u] * L::PK + c), q1 = pair(sq + (r0[u] + 8) * L::PK + c);
-      const float ak[4] = {k0.x, k1.x, k0.y, k1.y}, aq[4] = {q0.x, q1.x, q0.y, q1.y};
-      const float2 bb = pair(sk + (nt[u] * 8 + g) * L::PK + c);
-      if (IsExact<E>::value) {
-        mma(kk[u], ak, bb.x, bb.y);
-        mma(qk[u], aq, bb.x, bb.y);
-      } else {
+      for (int u = 0; u < 5; ++u) {
+        const int left = (r0[u] - g + (lane & 15)) * L::PK + kp * 16 + (lane >> 4) * 8;
+        const int right = (nt[u] * 8 + (lane & 7)) * L::PK + kp * 16 + ((lane >> 3) & 1) * 8;
+        uint32_t b0, b1;
+        asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];" : "=r"(b0), "=r"(b1) : "r"(smem_u32(sk + right)) : "memory");
+        mma_exact<E>(kk[u], four_tiles(sk + left), b0, b1);
+        mma_exact<E>(qk[u], four_tiles(sq + left), b0, b1);
+      }
+  } else {
+#pragma unroll 2
+    for (int ks = 0; ks < DK / 8; ++ks) {
+      const int c = ks * 8 + 2 * t;
+#pragma unroll
+      for (int u = 0; u < 5; ++u) {
+        const float2 k0 = pair(sk + r0[u] * L::PK + c), k1 = pair(sk + (r0[u] + 8) * L::PK + c);
+        const float2 q0 = pair(sq + r0[u] * L::PK + c), q1 = pair(sq + (r0[u] + 8) * L::PK + c);
+        const float ak[4] = {k0.x, k1.x, k0.y, k1.y}, aq[4] = {q0.x, q1.x, q0.y, q1.y};
+        const float2 bb = pair(sk + (nt[u] * 8 + g) * L::PK + c);
         float h[4], l[4];
         split4(ak, h, l);
         mma_split<false, 1>(kk + u, h, l, &bb);
@@ -127,6 +156,8 @@ __global__ void __launch_bounds__(128) prepare_kernel(Args a) {
       }
     }
   }
+  if (packs) bulk_read_wait();
+  __syncthreads();      // the tiles are free
   float* Tm = a.rec + ci * kRecord;
   float* Pm = Tm + kTri;
   float* Bm = BACK ? a.Bm + ci * kTri : nullptr;
@@ -149,7 +180,6 @@ __global__ void __launch_bounds__(128) prepare_kernel(Args a) {
         if (BACK) *reinterpret_cast<float2*>(Bm + at) = make_float2(m[0], m[1]);
       }
     }
-  if (packs) bulk_read_wait();    // T takes the tiles' place
   __syncthreads();
 
   // diagonal blocks of T: lane j solves column j of block `warp`
