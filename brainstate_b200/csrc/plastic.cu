@@ -20,24 +20,13 @@ static size_t workspace(const bsx_delta_t* d, bool backward) {
   return f * sizeof(float);
 }
 
-// Clears what lies behind each row's length in arrays of (batch, tokens, bytes of a token).
-struct Tails {
-  unsigned char* p[5];
-  int64_t token_bytes[5];
-  int n = 0;
-  void add(void* at, int64_t bytes) {
-    p[n] = static_cast<unsigned char*>(at);
-    token_bytes[n++] = bytes;
-  }
-};
-
-__global__ void __launch_bounds__(256) clear_tails_kernel(Args a, Tails tails) {
-  const int which = blockIdx.y % tails.n;
-  const int64_t per = tails.token_bytes[which];
-  for (int b = blockIdx.y / tails.n; b < a.B; b += gridDim.y / tails.n) {
+// Clears the outputs behind each row's length, `per` bytes a token (sequences that go token by token; the chunks of others
+// are cleared where they are prepared).
+__global__ void __launch_bounds__(256) clear_tails_kernel(Args a, int64_t per) {
+  for (int b = blockIdx.y; b < a.B; b += gridDim.y) {
     const int len = row_length(a, b);
     // whole elements of two bytes at least: to a 16-byte boundary, 16 bytes at a time, the rest
-    uint16_t* x = reinterpret_cast<uint16_t*>(tails.p[which] + ((int64_t)b * a.T + len) * per);
+    uint16_t* x = reinterpret_cast<uint16_t*>(static_cast<unsigned char*>(a.o) + ((int64_t)b * a.T + len) * per);
     const int64_t n = (a.T - len) * per / 2;
     int64_t head = ((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / 2;
     head = head < n ? head : n;
@@ -49,14 +38,6 @@ __global__ void __launch_bounds__(256) clear_tails_kernel(Args a, Tails tails) {
     const int64_t tail = head + body * 8 + first;
     if (first < 8 && tail < n) x[tail] = 0;
   }
-}
-
-static int clear_tails(const Args& a, const Tails& tails, cudaStream_t st) {
-  const int64_t most = 65535 / tails.n;
-  const dim3 grid(8, (unsigned)(tails.n * (a.B < most ? a.B : most)));
-  clear_tails_kernel<<<grid, 256, 0, st>>>(a, tails);
-  BSX_LAUNCH_CHECK("plastic clear_tails_kernel");
-  return BSX_OK;
 }
 
 static int check_sizes(const bsx_delta_t* d) {
@@ -75,11 +56,12 @@ static int check_sizes(const bsx_delta_t* d) {
   return BSX_OK;
 }
 
-static int clear_output_tails(const Args& a, int dtype, cudaStream_t st) {
+static int clear_tails(const Args& a, int dtype, cudaStream_t st) {
   if (!a.lengths) return BSX_OK;
-  Tails tails;
-  tails.add(a.o, (int64_t)a.Hv * a.dv * (dtype == BSX_T_F32 ? 4 : 2));
-  return clear_tails(a, tails, st);
+  const dim3 grid(8, (unsigned)(a.B < 65535 ? a.B : 65535));
+  clear_tails_kernel<<<grid, 256, 0, st>>>(a, (int64_t)a.Hv * a.dv * (dtype == BSX_T_F32 ? 4 : 2));
+  BSX_LAUNCH_CHECK("plastic clear_tails_kernel");
+  return BSX_OK;
 }
 
 static int fill(const bsx_delta_t* d, Args& a) {
@@ -162,7 +144,6 @@ extern "C" int bsx_delta_forward(const bsx_delta_t* d, void* out, float* state, 
   place(a, d, static_cast<float*>(ws), false);
   cudaStream_t st = as_stream(stream);
   if (a.NC > 0 && (rc = launch_prepare(a, d->dtype, false, st)) != BSX_OK) return rc;
-  if (a.NC > 0 && (rc = clear_output_tails(a, d->dtype, st)) != BSX_OK) return rc;
   return launch_scan(a, d->dtype, false, st);
 }
 
@@ -178,7 +159,7 @@ extern "C" int bsx_delta_recurrent(const bsx_delta_t* d, void* out, float* state
   a.o = out;
   a.state = state;
   cudaStream_t st = as_stream(stream);
-  if (a.T > 0 && (rc = clear_output_tails(a, d->dtype, st)) != BSX_OK) return rc;
+  if (a.T > 0 && (rc = clear_tails(a, d->dtype, st)) != BSX_OK) return rc;
   return launch_step(a, d->dtype, st);
 }
 
@@ -206,16 +187,6 @@ extern "C" int bsx_delta_backward(const bsx_delta_t* d, const void* dout, const 
   if (a.NC > 0) {
     if ((rc = launch_prepare(a, d->dtype, true, st)) != BSX_OK) return rc;
     if ((rc = launch_scan(a, d->dtype, true, st)) != BSX_OK) return rc;
-  }
-  if (a.NC > 0 && a.lengths) {
-    const int64_t size = d->dtype == BSX_T_F32 ? 4 : 2;
-    Tails tails;
-    tails.add(dq, a.Hk * a.dk * size);
-    tails.add(dk, a.Hk * a.dk * size);
-    tails.add(dv, a.Hv * a.dv * size);
-    tails.add(dg, a.Hv * 4);
-    tails.add(dbeta, a.Hv * 4);
-    if ((rc = clear_tails(a, tails, st)) != BSX_OK) return rc;
   }
   if ((rc = launch_backward_scan(a, d->dtype, st)) != BSX_OK) return rc;
   return a.NC > 0 ? launch_backward_chunks(a, d->dtype, st) : BSX_OK;

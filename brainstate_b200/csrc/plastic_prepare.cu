@@ -44,6 +44,38 @@ __device__ __forceinline__ uint4 four_tiles(const void* row) {
   return r;
 }
 
+// Clears this head's outputs (gradients) of a chunk's tokens from `live` on, which no later kernel writes.  Gradients of
+// shared keys are written whole where they are summed.
+template <typename E, bool BACK>
+__device__ __forceinline__ void clear_tail(const Args& a, int b, int h, int64_t t0, int live) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, end = (int)min((int64_t)kC, a.T - t0);
+  auto rows = [&](void* p, int width) {      // (batch, tokens, Hv, width)
+    constexpr int V = 16 / sizeof(E);
+    const bool wide = width % V == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+    for (int r = live + warp; r < end; r += 4) {
+      E* x = static_cast<E*>(p) + (((int64_t)b * a.T + t0 + r) * a.Hv + h) * width;
+      if (wide)
+        for (int c = lane; c < width / V; c += 32) reinterpret_cast<int4*>(x)[c] = make_int4(0, 0, 0, 0);
+      else
+        for (int c = lane; c < width; c += 32) x[c] = from_f<E>(0.f);
+    }
+  };
+  if (!BACK) {
+    rows(a.o, a.dv);
+    return;
+  }
+  rows(a.dv_, a.dv);
+  if (a.Hk == a.Hv) {
+    rows(a.dq, a.dk);
+    rows(a.dk_, a.dk);
+  }
+  for (int r = live + threadIdx.x; r < end; r += 128) {
+    const int64_t at = ((int64_t)b * a.T + t0 + r) * a.Hv + h;
+    a.dg[at] = 0.f;
+    a.dbeta[at] = 0.f;
+  }
+}
+
 template <typename E, int DK, bool BACK>
 __global__ void __launch_bounds__(128) prepare_kernel(Args a) {
   using L = PrepLayout<E, DK>;
@@ -62,8 +94,9 @@ __global__ void __launch_bounds__(128) prepare_kernel(Args a) {
   const int bh = blockIdx.x / a.NC, b = bh / a.Hv, h = bh - b * a.Hv, hk = h / (a.Hv / a.Hk);
   const int len = row_length(a, b);
   const int64_t t0 = (int64_t)chunk * kC;
-  if (t0 >= len) return;
-  const int rows = (int)min((int64_t)kC, len - t0);
+  const int rows = t0 < len ? (int)min((int64_t)kC, len - t0) : 0;
+  if (a.lengths && rows < kC) clear_tail<E, BACK>(a, b, h, t0, rows);
+  if (rows == 0) return;
   const int64_t ci = (int64_t)bh * a.NC + chunk;
 
   // g and beta first: their sums are a chain that starts with these loads

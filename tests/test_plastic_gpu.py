@@ -92,6 +92,25 @@ def test_padded_rows(cuda, dtype, T):
     assert torch.equal(got['state'][0].cpu(), args['initial'][0])
 
 
+@pytest.mark.parametrize('dtype', [F32, BF16, F16])
+@pytest.mark.parametrize('T,Hk,dk,dv', [(8, 2, 48, 40), (200, 1, 64, 48), (200, 2, 33, 20), (130, 2, 128, 132), (129, 1, 7, 9)])
+def test_everything_behind_a_length_is_written(cuda, dtype, T, Hk, dk, dv):
+    """With new memory full of NaN: outputs and gradients behind a length are zero, all others are finite and right."""
+    args = inputs(6, T, Hk, 2, dk, dv, dtype, seed=T + dk)
+    lengths = [0, 1, min(64, T), min(65, T), T - 1, T]
+    before = torch.are_deterministic_algorithms_enabled()
+    torch.use_deterministic_algorithms(True)       # fills what is allocated without a value
+    try:
+        assert torch.empty(64, device='cuda').isnan().all()
+        got, want = run_both(args, lengths)
+    finally:
+        torch.use_deterministic_algorithms(before)
+    compare(got, want)
+    for b, n in enumerate(lengths):
+        for name in ('o', 'dq', 'dk', 'dv', 'dg', 'dbeta'):
+            assert torch.all(got[name][b, n:] == 0), name
+
+
 def test_lengths_out_of_range_are_clipped(cuda):
     from brainstate_b200 import plastic
     args = {n: x.cuda() for n, x in inputs(3, 40, 1, 1, 16, 16, F32).items()}
